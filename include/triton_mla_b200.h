@@ -365,6 +365,62 @@ int tmla_linear(const TmlaLinearParams* p, void* stream);
    Host-only. */
 int64_t tmla_linear_workspace_bytes(int32_t m, int32_t n, int32_t k, int32_t groups, int32_t num_sms);
 
+/* ---------------------------------------------------------------- int8 projections (W8A8)
+   An MLA layer's projections with both operands in int8: a scale per token and a scale per
+   output channel, products summed exactly in int32.  No counterpart in the reference, whose
+   layer is 16-bit (model.py:101-124).  A layer step runs tmla_rms_norm_int8 ->
+   tmla_linear_int8 ([wq_a; wkv_a]), tmla_rms_norm_int8 (q_norm) -> tmla_linear_int8 (wq_b), and
+   tmla_quantize_int8 -> tmla_linear_int8 (wo) around the decode. */
+
+/* int8 rows with a scale each.  dtype (TMLA_DTYPE_*) is the type of x, residual, weight and h.
+   tmla_quantize_int8: scale[i] = max(max_j |x[i, j]| / 127, 2^-126), q[i, j] = x[i, j] / scale[i]
+   rounded to nearest (ties to even); weight and residual must be NULL.  Also for a weight
+   [n, k], whose rows are output channels.
+   tmla_rms_norm_int8: h = x + residual rounded to dtype (h = x without a residual; h is written
+   only with one), y = h * weight / sqrt(mean(h^2) + eps) in fp32, and y quantised as above.  h may
+   be x or residual themselves (same strides), not another overlap of them.
+   A row that holds a NaN or an infinity gets scale NaN and integers 0.  |q| <= 127 always.
+   Any m (below 2^31), k (1 to 2^30) and row strides >= k; rows that start on 16-byte boundaries (8 for q from a
+   16-bit x) are moved in whole vectors.  Bytes of q past k in a row are not written. */
+typedef struct TmlaInt8RowsParams {
+  const void* x;                   /* [m, k] */
+  int64_t x_stride;
+  const void* residual;            /* [m, k] or NULL */
+  int64_t residual_stride;
+  const void* weight;              /* [k] (norm only) */
+  void* h;                         /* [m, k], with a residual */
+  int64_t h_stride;
+  void* q;                         /* int8 [m, k] */
+  int64_t q_stride;
+  float* scale;                    /* [m] */
+  int64_t m;
+  int32_t k;
+  int32_t dtype;
+  float eps;
+  int32_t flags;                   /* TMLA_LAYER_FLAG_*: with PDL the preceding kernel must not write weight */
+} TmlaInt8RowsParams;
+int tmla_quantize_int8(const TmlaInt8RowsParams* p, void* stream);
+int tmla_rms_norm_int8(const TmlaInt8RowsParams* p, void* stream);
+
+/* y[i, j] = x_scale[i] * w_scale[j] * sum_c x[i, c] w[j, c], the sum exact in int32 (k at most
+   TMLA_LINEAR_INT8_MAX_K, the longest whose sum of (-128)^2 terms fits), one rounding to dtype
+   at the end (fp32 products of the sum and the scales).  Any m, n >= 0 and k >= 1. */
+#define TMLA_LINEAR_INT8_MAX_K 131071
+typedef struct TmlaLinearInt8Params {
+  const void* x;                   /* int8 [m, k] */
+  int64_t x_stride;
+  const float* x_scale;            /* [m] */
+  const void* w;                   /* int8 [n, k] */
+  int64_t w_stride;
+  const float* w_scale;            /* [n] */
+  void* y;                         /* [m, n] */
+  int64_t y_stride;
+  int32_t m, n, k;
+  int32_t dtype;                   /* TMLA_DTYPE_* of y */
+  int32_t flags;                   /* TMLA_LAYER_FLAG_* */
+} TmlaLinearInt8Params;
+int tmla_linear_int8(const TmlaLinearInt8Params* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,5 +1,6 @@
 // The decode registered as a PyTorch operator, torch.ops.triton_mla.decode, on top of the C ABI
-// (include/triton_mla_b200.h, tmla_decode).
+// (include/triton_mla_b200.h, tmla_decode), and the int8 projections (quantize_int8, rms_norm_int8,
+// linear_int8) beside it.
 //
 // The reference runs its decode as Python code around two Triton launches
 // (src/triton_mla/kernel.py:204-323), which torch.compile treats as opaque Python.  Here the
@@ -100,6 +101,147 @@ void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& le
               rc == TMLA_ERR_CUDA ? tmla_last_cuda_error() : "");
 }
 
+// ---------------------------------------------------------------- int8 projections
+// quantize_int8(x [m, k]) -> (q int8 [m, k], scale fp32 [m]); rms_norm_int8 -> (q, scale, h): h is a
+// new tensor when there is a residual and no residual_out, else empty; linear_int8(x_q [m, k],
+// x_scale [m], w_q [n, k], w_scale [n]) -> y [m, n] in out_dtype.  Rows of q start on 16-byte
+// boundaries (row stride k rounded up to 16), as linear_int8's TMA loads want them.  Outputs come
+// from the caching allocator, the launches go on the current stream of the inputs' device.
+
+// An [m, k] int8 tensor whose rows start on 16-byte boundaries.
+at::Tensor int8_rows(const at::Tensor& x) {
+  const int64_t m = x.size(0), k = x.size(1), stride = (k + 15) / 16 * 16;
+  return at::empty_strided({m, k}, {stride, 1}, x.options().dtype(at::kChar));
+}
+
+void check_rows(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda(), "triton_mla: CUDA tensors only (there is no CPU implementation), got ", what, " on ",
+              t.device());
+  TORCH_CHECK(t.dim() == 2 && (t.size(1) == 0 || t.stride(1) == 1), "triton_mla: ", what,
+              " must be a matrix with unit inner stride");
+}
+// A one-row matrix may carry any row stride; the library wants at least the row's length.
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+
+void check_rc(int rc, const char* what) {
+  TORCH_CHECK(rc == TMLA_OK, what, " failed: ", tmla_error_string(rc), " ",
+              rc == TMLA_ERR_CUDA ? tmla_last_cuda_error() : "");
+}
+
+TmlaInt8RowsParams rows_params(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, bool overlap) {
+  TmlaInt8RowsParams p = {};
+  TORCH_CHECK(x.size(1) <= INT32_MAX, "triton_mla: rows of at most 2^31 - 1 values");
+  p.x = x.data_ptr();
+  p.x_stride = row_stride(x);
+  p.q = q.data_ptr();
+  p.q_stride = row_stride(q);
+  p.scale = scale.data_ptr<float>();
+  p.m = x.size(0);
+  p.k = (int32_t)x.size(1);
+  p.dtype = dtype_code(x.scalar_type());
+  p.flags = overlap ? TMLA_LAYER_FLAG_PDL : 0;
+  return p;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_int8_cuda(const at::Tensor& x, bool overlap) {
+  check_rows(x, "x");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor q = int8_rows(x), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+  const TmlaInt8RowsParams p = rows_params(x, q, scale, overlap);
+  check_rc(tmla_quantize_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+           "tmla_quantize_int8");
+  return {q, scale};
+}
+std::tuple<at::Tensor, at::Tensor> quantize_int8_meta(const at::Tensor& x, bool) {
+  return {int8_rows(x), at::empty({x.size(0)}, x.options().dtype(at::kFloat))};
+}
+
+void check_like(const at::Tensor& t, const at::Tensor& x, const char* what) {
+  check_rows(t, what);
+  TORCH_CHECK(t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device(),
+              "triton_mla.rms_norm_int8: ", what, " must have x's shape, dtype and device");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_cuda(const at::Tensor& x, const at::Tensor& weight,
+                                                                  double eps,
+                                                                  const std::optional<at::Tensor>& residual,
+                                                                  const std::optional<at::Tensor>& residual_out,
+                                                                  bool overlap) {
+  check_rows(x, "x");
+  TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(1) && weight.is_contiguous() &&
+                  weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
+              "triton_mla.rms_norm_int8: weight must be a contiguous [k] vector of x's dtype and device");
+  TORCH_CHECK(!residual_out.has_value() || residual.has_value(),
+              "triton_mla.rms_norm_int8: residual_out without residual");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor q = int8_rows(x), scale = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), h;
+  TmlaInt8RowsParams p = rows_params(x, q, scale, overlap);
+  p.weight = weight.data_ptr();
+  p.eps = (float)eps;
+  if (residual.has_value()) {
+    check_like(*residual, x, "residual");
+    if (residual_out.has_value())
+      check_like(*residual_out, x, "residual_out");
+    else
+      h = at::empty({x.size(0), x.size(1)}, x.options());
+    const at::Tensor& out = residual_out.has_value() ? *residual_out : h;
+    p.residual = residual->data_ptr();
+    p.residual_stride = row_stride(*residual);
+    p.h = out.data_ptr();
+    p.h_stride = row_stride(out);
+  }
+  if (!h.defined()) h = at::empty({0}, x.options());
+  check_rc(tmla_rms_norm_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
+           "tmla_rms_norm_int8");
+  return {q, scale, h};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_meta(const at::Tensor& x, const at::Tensor&, double,
+                                                                  const std::optional<at::Tensor>& residual,
+                                                                  const std::optional<at::Tensor>& residual_out,
+                                                                  bool) {
+  at::Tensor h = residual.has_value() && !residual_out.has_value() ? at::empty({x.size(0), x.size(1)}, x.options())
+                                                                   : at::empty({0}, x.options());
+  return {int8_rows(x), at::empty({x.size(0)}, x.options().dtype(at::kFloat)), h};
+}
+
+at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w,
+                            const at::Tensor& w_scale, at::ScalarType out_dtype, bool overlap) {
+  check_rows(x, "x_q");
+  check_rows(w, "w_q");
+  TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar && x.size(1) == w.size(1) &&
+                  x.device() == w.device(),
+              "triton_mla.linear_int8: x_q [m, k] and w_q [n, k] must be int8 on one device");
+  TORCH_CHECK(x_scale.dim() == 1 && x_scale.size(0) == x.size(0) && w_scale.dim() == 1 &&
+                  w_scale.size(0) == w.size(0) && x_scale.scalar_type() == at::kFloat &&
+                  w_scale.scalar_type() == at::kFloat && x_scale.is_contiguous() && w_scale.is_contiguous() &&
+                  x_scale.device() == x.device() && w_scale.device() == x.device(),
+              "triton_mla.linear_int8: x_scale [m] and w_scale [n] must be contiguous fp32 vectors on x_q's device");
+  TORCH_CHECK(x.size(0) <= INT32_MAX && w.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX,
+              "triton_mla.linear_int8: sizes beyond 2^31 - 1");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
+  TmlaLinearInt8Params p = {};
+  p.x = x.data_ptr();
+  p.x_stride = row_stride(x);
+  p.x_scale = x_scale.data_ptr<float>();
+  p.w = w.data_ptr();
+  p.w_stride = row_stride(w);
+  p.w_scale = w_scale.data_ptr<float>();
+  p.y = y.data_ptr();
+  p.y_stride = w.size(0);
+  p.m = (int32_t)x.size(0);
+  p.n = (int32_t)w.size(0);
+  p.k = (int32_t)x.size(1);
+  p.dtype = dtype_code(out_dtype);
+  p.flags = overlap ? TMLA_LAYER_FLAG_PDL : 0;
+  check_rc(tmla_linear_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), "tmla_linear_int8");
+  return y;
+}
+at::Tensor linear_int8_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
+                            at::ScalarType out_dtype, bool) {
+  return at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
+}
+
 // Shapes only: out and lse are written in place, so there is nothing to return.
 void decode_meta(const at::Tensor&, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
                  const at::Tensor&, const at::Tensor&, int64_t, double, int64_t, int64_t,
@@ -111,8 +253,32 @@ TORCH_LIBRARY(triton_mla, m) {
   m.def(
       "decode(Tensor q, Tensor kv_cache, Tensor cache_seqlens, Tensor? block_table, Tensor(a!) out, "
       "Tensor(b!) lse, int num_splits, float softmax_scale, int kernel, int q_len, Tensor? status) -> ()");
+  m.def("quantize_int8(Tensor x, bool overlap) -> (Tensor, Tensor)");
+  m.def(
+      "rms_norm_int8(Tensor x, Tensor weight, float eps, Tensor? residual, Tensor(a!)? residual_out, bool overlap) "
+      "-> (Tensor, Tensor, Tensor)");
+  m.def(
+      "linear_int8(Tensor x_q, Tensor x_scale, Tensor w_q, Tensor w_scale, ScalarType out_dtype, bool overlap) "
+      "-> Tensor");
 }
 
-TORCH_LIBRARY_IMPL(triton_mla, CUDA, m) { m.impl("decode", &decode_cuda); }
+TORCH_LIBRARY_IMPL(triton_mla, CUDA, m) {
+  m.impl("decode", &decode_cuda);
+  m.impl("quantize_int8", &quantize_int8_cuda);
+  m.impl("rms_norm_int8", &rms_norm_int8_cuda);
+  m.impl("linear_int8", &linear_int8_cuda);
+}
 
-TORCH_LIBRARY_IMPL(triton_mla, Meta, m) { m.impl("decode", &decode_meta); }
+TORCH_LIBRARY_IMPL(triton_mla, Meta, m) {
+  m.impl("decode", &decode_meta);
+  m.impl("quantize_int8", &quantize_int8_meta);
+  m.impl("rms_norm_int8", &rms_norm_int8_meta);
+  m.impl("linear_int8", &linear_int8_meta);
+}
+
+// Serving operators: no gradient passes through them (their outputs require none).
+TORCH_LIBRARY_IMPL(triton_mla, Autograd, m) {
+  m.impl("quantize_int8", torch::CppFunction::makeFallthrough());
+  m.impl("rms_norm_int8", torch::CppFunction::makeFallthrough());
+  m.impl("linear_int8", torch::CppFunction::makeFallthrough());
+}

@@ -27,6 +27,7 @@ MAX_BATCH = 65535  # requests (and splits) of one decode call
 LAYER_FLAG_PDL = 1
 LINEAR_FLAG_TEST_STALL = 0x100
 LINEAR_MAX_TILES = 65536
+LINEAR_INT8_MAX_K = 131071
 W_NK = 0
 W_KN = 1
 KV_SAME = 0
@@ -72,6 +73,9 @@ EXPORTED = (
     "tmla_plan_units_device",
     "tmla_linear",
     "tmla_linear_workspace_bytes",
+    "tmla_quantize_int8",
+    "tmla_rms_norm_int8",
+    "tmla_linear_int8",
 )
 
 
@@ -221,6 +225,48 @@ class TmlaLinearParams(ctypes.Structure):
     ]
 
 
+class TmlaInt8RowsParams(ctypes.Structure):
+    """Mirror of ``TmlaInt8RowsParams``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("h", ctypes.c_void_p),
+        ("h_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64),
+        ("scale", ctypes.c_void_p),
+        ("m", ctypes.c_int64),
+        ("k", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("flags", ctypes.c_int32),
+    ]
+
+
+class TmlaLinearInt8Params(ctypes.Structure):
+    """Mirror of ``TmlaLinearInt8Params``."""
+
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("x_scale", ctypes.c_void_p),
+        ("w", ctypes.c_void_p),
+        ("w_stride", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("y_stride", ctypes.c_int64),
+        ("m", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("k", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+    ]
+
+
 class LibraryError(RuntimeError):
     """A non-zero return code from the C ABI."""
 
@@ -281,7 +327,9 @@ def load() -> ctypes.CDLL:
     lib.tmla_linear_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
     lib.tmla_linear_workspace_bytes.restype = i64
     for name, st in (("tmla_q_absorb_rope", TmlaQPrepParams), ("tmla_kv_norm_rope_append", TmlaKvAppendParams),
-                     ("tmla_o_unabsorb", TmlaOUnabsorbParams), ("tmla_linear", TmlaLinearParams)):
+                     ("tmla_o_unabsorb", TmlaOUnabsorbParams), ("tmla_linear", TmlaLinearParams),
+                     ("tmla_quantize_int8", TmlaInt8RowsParams), ("tmla_rms_norm_int8", TmlaInt8RowsParams),
+                     ("tmla_linear_int8", TmlaLinearInt8Params)):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(st), vp]
         fn.restype = ctypes.c_int

@@ -7,6 +7,9 @@ They replace the PyTorch glue of the reference's ``MLA.forward``
 (src/triton_mla/model.py:74-94 and 111-123): RoPE of q_pe and k_pe, kv_norm, the
 paged-cache append, the absorption einsums by W_UK / W_UV and the concatenation;
 and, for decode batches of up to 64 tokens, the projections' GEMMs (model.py:104-108, 124).
+
+For layers served with int8 weights and activations (no counterpart in the reference) there
+are ``quantize_int8``, ``rms_norm_int8`` and ``linear_int8``.
 """
 
 from __future__ import annotations
@@ -16,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernel import _DTYPE_CODES, _status_word
+from .kernel import _DTYPE_CODES, _require_cuda, _status_word
 
 
 def _stream(t: torch.Tensor):
@@ -214,3 +217,69 @@ def l2_prefetch(t: torch.Tensor, chunk_bytes: int = None, stride_bytes: int = No
     assert t.is_cuda and 0 < chunk and stride >= chunk and (count - 1) * stride + chunk <= nbytes
     _lib.check(_lib.load().tmla_l2_prefetch(ctypes.c_void_p(t.data_ptr()), chunk, stride, int(count), int(ctas),
                                              _stream(t)), "tmla_l2_prefetch")
+
+
+# ----------------------------------------------------------------------------- int8 projections
+def _int8_source(x: torch.Tensor) -> None:
+    _require_cuda(x)
+    assert x.dim() == 2 and x.shape[1] > 0, "a matrix [m, k] with k >= 1"
+    assert x.stride(1) == 1 or x.shape[1] == 1, "rows need unit inner stride"
+    if x.dtype not in _DTYPE_CODES:
+        raise TypeError(f"unsupported dtype {x.dtype}; use bfloat16, float16 or float32")
+
+
+def quantize_int8(x: torch.Tensor, overlap: bool = False):
+    """int8 rows of ``x`` [m, k] with one scale each: ``(q, scale)`` with q int8 [m, k], scale
+    fp32 [m] and ``x ~ q * scale[:, None]`` (C ABI: ``tmla_quantize_int8``).
+
+    scale = max(max |row| / 127, 2^-126); q = row / scale rounded to nearest.  For activations
+    (a scale per token) and for weights [n, k] (a scale per output channel).  A row with a NaN
+    or an infinity gets scale NaN and zeros.  Rows of q start on 16-byte boundaries, so q's row
+    stride is k rounded up to 16 (the padding bytes are not written).  Bf16, fp16 or fp32, any
+    row stride; no gradient.  ``overlap`` as in ``q_absorb_rope``."""
+    _int8_source(x)
+    return torch.ops.triton_mla.quantize_int8(x, overlap)
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                  residual: torch.Tensor | None = None, residual_out: torch.Tensor | None = None,
+                  overlap: bool = False):
+    """RMS norm of the residual stream with an int8 output: ``(q, scale, h)`` (C ABI:
+    ``tmla_rms_norm_int8``).
+
+    ``h = x + residual`` rounded to x's dtype, ``y = h * weight / sqrt(mean(h^2) + eps)`` in fp32,
+    and y's rows quantised as in ``quantize_int8``.  x [m, k] (any row stride), weight [k].  h is
+    the new residual: a new tensor, or ``residual_out``, which may be ``residual`` or ``x`` itself.
+    Without a residual h is None and x is normalised as it is.  ``overlap`` as in
+    ``q_absorb_rope`` (the preceding kernel must not write ``weight``)."""
+    _int8_source(x)
+    _require_cuda(weight, residual, residual_out)
+    assert weight.shape == (x.shape[1],) and weight.dtype == x.dtype and weight.is_contiguous()
+    assert weight.device == x.device
+    for t in (residual, residual_out):
+        if t is not None:
+            assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device
+            assert t.stride(1) == 1 or t.shape[1] == 1
+    assert residual is not None or residual_out is None, "residual_out without a residual"
+    q, scale, h = torch.ops.triton_mla.rms_norm_int8(x, weight, eps, residual, residual_out, overlap)
+    if residual is None:
+        return q, scale, None
+    return q, scale, (h if residual_out is None else residual_out)
+
+
+def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor,
+                out_dtype: torch.dtype = torch.bfloat16, overlap: bool = False) -> torch.Tensor:
+    """``(x_q * x_scale[:, None]) @ (w_q * w_scale[:, None]).T`` for int8 x_q [m, k] and w_q [n, k]
+    with fp32 scales per token and per output channel, as ``quantize_int8`` and ``rms_norm_int8``
+    give them (C ABI: ``tmla_linear_int8``).  The products are summed exactly (int32, k at most
+    131071) and scaled in fp32; y [m, n] is rounded once to ``out_dtype`` (bf16, fp16 or fp32).
+    Any m and n.  ``overlap`` as in ``linear`` (the preceding kernel must not write ``w_q``)."""
+    _require_cuda(x_q, x_scale, w_q, w_scale)
+    assert x_q.dim() == 2 and w_q.dim() == 2 and x_q.shape[1] == w_q.shape[1] and x_q.shape[1] > 0
+    assert x_q.dtype == torch.int8 and w_q.dtype == torch.int8, "int8 operands"
+    assert x_scale.shape == x_q.shape[:1] and w_scale.shape == w_q.shape[:1], "a scale per token and per channel"
+    assert x_scale.dtype == torch.float32 and w_scale.dtype == torch.float32
+    assert x_q.shape[1] <= _lib.LINEAR_INT8_MAX_K, "the int32 sum of a longer k can overflow"
+    if out_dtype not in _DTYPE_CODES:
+        raise TypeError(f"unsupported out_dtype {out_dtype}; use bfloat16, float16 or float32")
+    return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap)
