@@ -10,9 +10,12 @@
 // output written exactly once.  Arithmetic is fp32 whatever T is; h is rounded to T first (the
 // norm is of the residual stream as stored), the int8 values are rounded once, to nearest even.
 //
+// Bound: HBM bandwidth.  Measured on B200 (inputs beyond L2, back to back): quantise 8192 x 7168 bf16
+// 28.4 us (6.2 TB/s, 95% of a copy), norm with residual 69.9 us (5.9 TB/s, 90%), norm without
+// 40.5 us; one token 2.0-2.7 us, which is launch and one trip to memory.
+//
 // A row that holds a NaN or an infinity has no scale: its scale is NaN and its integers are 0,
-// so every product with it is NaN.  The maximum is taken over the bit patterns of |y| as
-// unsigned integers, in which NaN > inf > finite.
+// so every product with it is NaN.  The maximum keeps a NaN.
 #include "tmla_common.cuh"
 #include "tmla_ptx.cuh"
 
@@ -37,8 +40,6 @@ struct Args {
   int64_t m;
   int k;
   float eps;
-  // Whether each tensor's rows are aligned for whole-vector accesses.
-  bool x_vec, r_vec, w_vec, h_vec, q_vec;
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -48,38 +49,52 @@ __device__ __forceinline__ void from_float(float v, float& o) { o = v; }
 __device__ __forceinline__ void from_float(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void from_float(float v, __half& o) { o = __float2half_rn(v); }
 
-// 16 bytes of T.
+// The values of a 16-byte vector of T, and back with one rounding each.
 template <typename T>
-struct alignas(16) Vec {
-  static constexpr int N = 16 / sizeof(T);
-  T e[N];
-};
+constexpr int kPer = 16 / (int)sizeof(T);
 
-// Elements [at, at + N) of a row of k, zeros past its end.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* row, int at, int k, bool aligned) {
-  Vec<T> v;
-  if (aligned && at + Vec<T>::N <= k) {
-    v = *reinterpret_cast<const Vec<T>*>(row + at);
-  } else {
-#pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j) {
-      if (at + j < k)
-        v.e[j] = row[at + j];
-      else
-        from_float(0.f, v.e[j]);
-    }
-  }
-  return v;
+__device__ __forceinline__ void unpack2(uint32_t w, const __nv_bfloat16*, float& a, float& b) {
+  a = __uint_as_float(w << 16);
+  b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t w, const __half*, float& a, float& b) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  a = f.x, b = f.y;
 }
 template <typename T>
-__device__ __forceinline__ void store_vec(T* row, int at, int k, bool aligned, const Vec<T>& v) {
-  if (aligned && at + Vec<T>::N <= k) {
-    *reinterpret_cast<Vec<T>*>(row + at) = v;
+__device__ __forceinline__ void unpack(uint4 u, float (&v)[kPer<T>]) {
+  if constexpr (sizeof(T) == 4) {
+    v[0] = __uint_as_float(u.x), v[1] = __uint_as_float(u.y);
+    v[2] = __uint_as_float(u.z), v[3] = __uint_as_float(u.w);
   } else {
+    const T* t = nullptr;
+    unpack2(u.x, t, v[0], v[1]);
+    unpack2(u.y, t, v[2], v[3]);
+    unpack2(u.z, t, v[4], v[5]);
+    unpack2(u.w, t, v[6], v[7]);
+  }
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// T(x + r), element by element.
+template <typename T>
+__device__ __forceinline__ uint4 add(uint4 x, uint4 r) {
+  float a[kPer<T>], b[kPer<T>];
+  unpack<T>(x, a);
+  unpack<T>(r, b);
 #pragma unroll
-    for (int j = 0; j < Vec<T>::N; ++j)
-      if (at + j < k) row[at + j] = v.e[j];
+  for (int j = 0; j < kPer<T>; ++j) a[j] += b[j];
+  if constexpr (sizeof(T) == 4) {
+    return make_uint4(__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(a[2]), __float_as_uint(a[3]));
+  } else {
+    const T* t = nullptr;
+    return make_uint4(pack2(a[0], a[1], t), pack2(a[2], a[3], t), pack2(a[4], a[5], t), pack2(a[6], a[7], t));
   }
 }
 
@@ -91,7 +106,7 @@ __device__ __forceinline__ uint32_t round_bits(float v, float inv) {
 // The integers of N = 4 or 8 values.  |v * inv| <= 127 (1 + 2^-22) by the choice of the scale, so no
 // value rounds beyond 127.
 template <int N>
-__device__ __forceinline__ void store_q(int8_t* row, int at, int k, bool aligned, const float (&v)[N], float inv) {
+__device__ __forceinline__ void store_q(int8_t* q, const float (&v)[N], float inv) {
   uint32_t w[N / 4];
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
@@ -99,22 +114,25 @@ __device__ __forceinline__ void store_q(int8_t* row, int at, int k, bool aligned
     const uint32_t hi = __byte_perm(round_bits(v[4 * j + 2], inv), round_bits(v[4 * j + 3], inv), 0x0040);
     w[j] = __byte_perm(lo, hi, 0x5410);
   }
-  if (aligned && at + N <= k) {
-    if constexpr (N == 8)
-      *reinterpret_cast<uint2*>(row + at) = make_uint2(w[0], w[1]);
-    else
-      *reinterpret_cast<uint32_t*>(row + at) = w[0];
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (at + j < k) row[at + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
-  }
+  if constexpr (N == 8)
+    *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+  else
+    *reinterpret_cast<uint32_t*>(q) = w[0];
 }
 
-// Maximum of `mx` and, with the norm, sum of `sum` over the threads of a row (whole warps).
+// The larger of two values that are not negative; NaN if one of them is NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// Maximum of `top` (not negative, or NaN: bit patterns order them, NaN > inf > finite) and, with the
+// norm, sum of `sum` over the threads of a row (whole warps).
 template <bool kNorm>
-__device__ __forceinline__ void reduce_row(uint32_t& mx, float& sum, uint32_t (*s_mx)[32], float (*s_sum)[32]) {
-  mx = __reduce_max_sync(0xffffffffu, mx);
+__device__ __forceinline__ void reduce_row(float& top, float& sum, uint32_t (*s_mx)[32], float (*s_sum)[32]) {
+  uint32_t mx = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  top = __uint_as_float(mx);
   if constexpr (kNorm) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -127,7 +145,7 @@ __device__ __forceinline__ void reduce_row(uint32_t& mx, float& sum, uint32_t (*
     if constexpr (kNorm) s_sum[threadIdx.y][warp] = sum;
   }
   __syncthreads();
-  mx = __reduce_max_sync(0xffffffffu, lane < warps ? s_mx[threadIdx.y][lane] : 0u);
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? s_mx[threadIdx.y][lane] : 0u));
   if constexpr (kNorm) {
     sum = lane < warps ? s_sum[threadIdx.y][lane] : 0.f;
 #pragma unroll
@@ -137,10 +155,10 @@ __device__ __forceinline__ void reduce_row(uint32_t& mx, float& sum, uint32_t (*
 
 // From the row's max |h w| (bits) and sum of squares: the scale, and the factors of h w.
 template <bool kNorm>
-__device__ __forceinline__ void row_scale(uint32_t mx, float sum, int k, float eps, float& scale, float& rstd,
+__device__ __forceinline__ void row_scale(float mx, float sum, int k, float eps, float& scale, float& rstd,
                                           float& inv) {
   rstd = kNorm ? rsqrtf(sum / (float)k + eps) : 1.f;
-  const float top = __uint_as_float(mx) * rstd;
+  const float top = mx * rstd;
   if (!(top < INFINITY)) {  // a NaN or an infinity in the row (or y beyond fp32)
     scale = __uint_as_float(0x7fc00000u);
     inv = 0.f;
@@ -150,134 +168,167 @@ __device__ __forceinline__ void row_scale(uint32_t mx, float sum, int k, float e
   inv = 1.f / scale;
 }
 
-// h = T(x + r) of one vector, as floats; written to h when there is a residual.
-template <typename T>
-__device__ __forceinline__ void add_residual(Vec<T>& x, const Vec<T>& r) {
-#pragma unroll
-  for (int j = 0; j < Vec<T>::N; ++j) from_float(to_float(x.e[j]) + to_float(r.e[j]), x.e[j]);
+// The row's running maximum of |y| (up to rstd) and sum of squares over one value.
+template <bool kNorm>
+__device__ __forceinline__ float visit(float h, float w, float& mx, float& sum) {
+  if constexpr (kNorm) {
+    sum += h * h;
+    h *= w;
+  }
+  mx = max_nan(mx, fabsf(h));
+  return h;
 }
 
-// blockDim = (threads per row, rows per block).  Each thread holds kVecs vectors of its row:
-// vector i of thread t is number i * threads + t.
+// Rows on 16-byte boundaries.  blockDim = (threads per row, rows per block); each thread holds up
+// to kVecs vectors of its row, vector i of thread t being number i * threads + t, and the first
+// k % N threads one value each of the row's end.  Loads are predicated, not branched around, so
+// that all of a thread's are in flight at once.  The row stays packed in T across the reduction (4
+// registers per vector); h w is formed again after it.
 template <typename T, int kVecs, bool kNorm>
-__global__ void __launch_bounds__(kMaxThreads) rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kVecs >= 4 ? 512 : kMaxThreads, kVecs == 4 ? 2 : 1) rows_kernel(const Args a) {
   __shared__ uint32_t s_mx[32][32];
   __shared__ float s_sum[kNorm ? 32 : 1][32];
-  constexpr int N = Vec<T>::N;
+  constexpr int N = kPer<T>;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  const bool live = row < a.m;
-  const int threads = blockDim.x;
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  Vec<T> w[kNorm ? kVecs : 1];
+  const int threads = blockDim.x, t = threadIdx.x;
+  const int vecs = row < a.m ? a.k / N : 0;
+  const int last = row < a.m && t < a.k % N ? a.k - a.k % N + t : -1;  // this thread's value of the row's end
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 w[kNorm ? kVecs : 1];
+  float w_last = 0.f;
   if constexpr (kNorm) {
+    const T* wp = static_cast<const T*>(a.w);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
-      w[i] = load_vec(static_cast<const T*>(a.w), (i * threads + (int)threadIdx.x) * N, a.k, a.w_vec);
+      w[i] = i * threads + t < vecs ? reinterpret_cast<const uint4*>(wp)[i * threads + t] : zero;
+    if (last >= 0) w_last = to_float(wp[last]);
   }
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  float v[kVecs][N];
-  uint32_t mx = 0;
-  float sum = 0.f;
-  if (live) {
-    Vec<T> xv[kVecs];
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  uint4 h[kVecs];
+  float h_last = 0.f;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) xv[i] = load_vec(x, (i * threads + (int)threadIdx.x) * N, a.k, a.x_vec);
-    if (kNorm && a.r != nullptr) {
-      const T* r = static_cast<const T*>(a.r) + row * a.r_stride;
-      T* h = static_cast<T*>(a.h) + row * a.h_stride;
-      Vec<T> rv[kVecs];
+  for (int i = 0; i < kVecs; ++i)
+    h[i] = i * threads + t < vecs ? reinterpret_cast<const uint4*>(x)[i * threads + t] : zero;
+  if (last >= 0) h_last = to_float(x[last]);
+  if (kNorm && a.r != nullptr) {
+    const T* r = static_cast<const T*>(a.r) + row * a.r_stride;
+    T* out = static_cast<T*>(a.h) + row * a.h_stride;
+    uint4 rv[kVecs];
 #pragma unroll
-      for (int i = 0; i < kVecs; ++i) rv[i] = load_vec(r, (i * threads + (int)threadIdx.x) * N, a.k, a.r_vec);
-#pragma unroll
-      for (int i = 0; i < kVecs; ++i) {
-        add_residual(xv[i], rv[i]);
-        store_vec(h, (i * threads + (int)threadIdx.x) * N, a.k, a.h_vec, xv[i]);
-      }
-    }
+    for (int i = 0; i < kVecs; ++i)
+      rv[i] = i * threads + t < vecs ? reinterpret_cast<const uint4*>(r)[i * threads + t] : zero;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float f = to_float(xv[i].e[j]);
-        if constexpr (kNorm) {
-          sum += f * f;
-          f *= to_float(w[i].e[j]);
-        }
-        v[i][j] = f;
-        mx = max(mx, __float_as_uint(f) & 0x7fffffffu);
-      }
+      h[i] = add<T>(h[i], rv[i]);
+      if (i * threads + t < vecs) reinterpret_cast<uint4*>(out)[i * threads + t] = h[i];
+    }
+    if (last >= 0) {
+      T v;
+      from_float(h_last + to_float(r[last]), v);
+      out[last] = v;
+      h_last = to_float(v);
     }
   }
-  reduce_row<kNorm>(mx, sum, s_mx, s_sum);
-  if (!live) return;
-  float scale, rstd, inv;
-  row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
-  if (threadIdx.x == 0) a.scale[row] = scale;
-  int8_t* q = a.q + row * a.q_stride;
+  float mx = 0.f, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kVecs; ++i) {
-    const int at = (i * threads + (int)threadIdx.x) * N;
-    if (at >= a.k) break;
+    float hv[N], wv[N];
+    unpack<T>(h[i], hv);
+    if constexpr (kNorm) unpack<T>(w[i], wv);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[i][j] = inv == 0.f ? 0.f : (kNorm ? v[i][j] * rstd : v[i][j]);
-    store_q(q, at, a.k, a.q_vec, v[i], inv);
+    for (int j = 0; j < N; ++j) visit<kNorm>(hv[j], kNorm ? wv[j] : 1.f, mx, sum);
   }
+  h_last = visit<kNorm>(h_last, w_last, mx, sum);
+  reduce_row<kNorm>(mx, sum, s_mx, s_sum);
+  if (row >= a.m) return;
+  float scale, rstd, inv;
+  row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
+  if (t == 0) a.scale[row] = scale;
+  int8_t* q = a.q + row * a.q_stride;
+  const bool bad = inv == 0.f;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    if (i * threads + t >= vecs) break;
+    float hv[N], wv[N];
+    unpack<T>(h[i], hv);
+    if constexpr (kNorm) unpack<T>(w[i], wv);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if constexpr (kNorm) hv[j] = hv[j] * wv[j] * rstd;
+      if (bad) hv[j] = 0.f;
+    }
+    store_q(q + (i * threads + t) * N, hv, inv);
+  }
+  if (last >= 0) q[last] = (int8_t)round_bits(bad ? 0.f : (kNorm ? h_last * rstd : h_last), inv);
 }
 
-// Rows too long for the registers of a block: the row is read a second time (from L2) for its
-// integers.  With a residual the second pass reads h, which the same thread has written.
-template <typename T, bool kNorm>
-__global__ void __launch_bounds__(kMaxThreads) long_rows_kernel(const Args a) {
+// Rows that do not start on 16-byte boundaries, value by value, and rows too long for the registers of
+// a block: the row is read a second time (from L1 / L2) for its integers.  With a residual the
+// second pass reads h, which the same thread has written.
+template <typename T, bool kNorm, bool kAligned>
+__global__ void __launch_bounds__(kMaxThreads) loop_kernel(const Args a) {
   __shared__ uint32_t s_mx[1][32];
   __shared__ float s_sum[1][32];
-  constexpr int N = Vec<T>::N;
+  constexpr int N = kPer<T>;
   const int64_t row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* r = static_cast<const T*>(a.r) + row * a.r_stride;
   T* h = static_cast<T*>(a.h) + row * a.h_stride;
   const T* w = static_cast<const T*>(a.w);
   const bool res = kNorm && a.r != nullptr;
+  const int vecs = kAligned ? a.k / N : 0;  // the first values as whole vectors, the others one by one
+  const int step = blockDim.x;
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
-  const int step = (int)blockDim.x * N;
-  uint32_t mx = 0;
-  float sum = 0.f;
-  for (int64_t at = (int64_t)threadIdx.x * N; at < a.k; at += step) {
-    Vec<T> xv = load_vec(x, (int)at, a.k, a.x_vec);
+  float mx = 0.f, sum = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < vecs; i += step) {
+    uint4 u = reinterpret_cast<const uint4*>(x)[i];
     if (res) {
-      add_residual(xv, load_vec(r, (int)at, a.k, a.r_vec));
-      store_vec(h, (int)at, a.k, a.h_vec, xv);
+      u = add<T>(u, reinterpret_cast<const uint4*>(r)[i]);
+      reinterpret_cast<uint4*>(h)[i] = u;
     }
-    Vec<T> wv;
-    if constexpr (kNorm) wv = load_vec(w, (int)at, a.k, a.w_vec);
+    float hv[N], wv[N];
+    unpack<T>(u, hv);
+    if constexpr (kNorm) unpack<T>(reinterpret_cast<const uint4*>(w)[i], wv);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      float f = to_float(xv.e[j]);
-      if constexpr (kNorm) {
-        sum += f * f;
-        f *= to_float(wv.e[j]);
-      }
-      mx = max(mx, __float_as_uint(f) & 0x7fffffffu);
+    for (int j = 0; j < N; ++j) visit<kNorm>(hv[j], kNorm ? wv[j] : 1.f, mx, sum);
+  }
+#pragma unroll 4
+  for (int j = vecs * N + (int)threadIdx.x; j < a.k; j += step) {
+    T v = x[j];
+    if (res) {
+      from_float(to_float(v) + to_float(r[j]), v);
+      h[j] = v;
     }
+    visit<kNorm>(to_float(v), kNorm ? to_float(w[j]) : 1.f, mx, sum);
   }
   reduce_row<kNorm>(mx, sum, s_mx, s_sum);
   float scale, rstd, inv;
   row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
   if (threadIdx.x == 0) a.scale[row] = scale;
   int8_t* q = a.q + row * a.q_stride;
-  for (int64_t at = (int64_t)threadIdx.x * N; at < a.k; at += step) {
-    const Vec<T> xv = res ? load_vec<T>(h, (int)at, a.k, a.h_vec) : load_vec(x, (int)at, a.k, a.x_vec);
-    Vec<T> wv;
-    if constexpr (kNorm) wv = load_vec(w, (int)at, a.k, a.w_vec);
-    float v[N];
+  const T* src = res ? h : x;
+  const bool bad = inv == 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < vecs; i += step) {
+    float hv[N], wv[N];
+    unpack<T>(reinterpret_cast<const uint4*>(src)[i], hv);
+    if constexpr (kNorm) unpack<T>(reinterpret_cast<const uint4*>(w)[i], wv);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      v[j] = to_float(xv.e[j]);
-      if constexpr (kNorm) v[j] = v[j] * to_float(wv.e[j]) * rstd;
-      if (inv == 0.f) v[j] = 0.f;
+      if constexpr (kNorm) hv[j] = hv[j] * wv[j] * rstd;
+      if (bad) hv[j] = 0.f;
     }
-    store_q(q, (int)at, a.k, a.q_vec, v, inv);
+    store_q(q + i * N, hv, inv);
+  }
+#pragma unroll 4
+  for (int j = vecs * N + (int)threadIdx.x; j < a.k; j += step) {
+    float v = to_float(src[j]);
+    if constexpr (kNorm) v = v * to_float(w[j]) * rstd;
+    q[j] = (int8_t)round_bits(bad ? 0.f : v, inv);
   }
 }
 
@@ -298,17 +349,29 @@ cudaError_t launch(K kernel, dim3 grid, dim3 block, const Args& a, bool pdl, cud
 }
 
 template <typename T, bool kNorm>
-cudaError_t run(const Args& a, bool pdl, cudaStream_t stream) {
-  constexpr int N = Vec<T>::N;
-  constexpr int kMaxVecs = 4;
-  const int64_t vecs = ((int64_t)a.k + N - 1) / N;
-  if (vecs > (int64_t)kMaxVecs * kMaxThreads)
-    return launch(long_rows_kernel<T, kNorm>, dim3((unsigned)a.m), dim3(kMaxThreads), a, pdl, stream);
-  const int per = vecs <= kMaxThreads ? 1 : kMaxVecs;
-  const int threads = (int)((vecs + 32 * per - 1) / (32 * per) * 32);
-  const dim3 grid((unsigned)a.m), block(threads, 1);
-  return per == 1 ? launch(rows_kernel<T, 1, kNorm>, grid, block, a, pdl, stream)
-                  : launch(rows_kernel<T, kMaxVecs, kNorm>, grid, block, a, pdl, stream);
+cudaError_t run(const Args& a, bool aligned, bool pdl, cudaStream_t stream) {
+  const int vecs = a.k / kPer<T> > 0 ? a.k / kPer<T> : 1;
+  if (!aligned || vecs > 8 * 512) {
+    const int threads = a.k < kMaxThreads ? (a.k + 31) / 32 * 32 : kMaxThreads;
+    return aligned ? launch(loop_kernel<T, kNorm, true>, dim3((unsigned)a.m), dim3(threads), a, pdl, stream)
+                   : launch(loop_kernel<T, kNorm, false>, dim3((unsigned)a.m), dim3(threads), a, pdl, stream);
+  }
+  // Vectors per thread (bf16 on B200, us per call): 4 keep more loads in flight than 1 or 2 (norm with
+  // residual of 8192 x 7168: 72.7 against 98.3 and 96.1; 4096 x 16384: 84.7 against 115), and 8
+  // leave registers for half the warps (105.5).  Below 128 vectors a row is one warp or less
+  // with 4 per thread, so 2 (65536 x 512, quantise: 19.0 against 22.1) or 1 fill it.  Rows of
+  // less than 128 threads share a block (24576 x 1536: 20.0 with 128 threads, 22.2 with 256,
+  // 25.9 with 64).
+  const int per = vecs > 4 * 512 ? 8 : vecs >= 128 ? 4 : vecs >= 64 ? 2 : 1;
+  const int threads = (vecs + 32 * per - 1) / (32 * per) * 32;
+  const int rows = threads >= 128 ? 1 : 128 / threads;
+  const dim3 grid((unsigned)((a.m + rows - 1) / rows)), block(threads, rows);
+  switch (per) {
+    case 1: return launch(rows_kernel<T, 1, kNorm>, grid, block, a, pdl, stream);
+    case 2: return launch(rows_kernel<T, 2, kNorm>, grid, block, a, pdl, stream);
+    case 4: return launch(rows_kernel<T, 4, kNorm>, grid, block, a, pdl, stream);
+    default: return launch(rows_kernel<T, 8, kNorm>, grid, block, a, pdl, stream);
+  }
 }
 
 bool rows_aligned(const void* p, int64_t stride, int size, int bytes) {
@@ -341,23 +404,23 @@ int start(const TmlaInt8RowsParams& p, bool norm, void* stream) {
   a.m = p.m;
   a.k = p.k;
   a.eps = p.eps;
-  a.x_vec = rows_aligned(p.x, p.x_stride, size, 16);
-  a.r_vec = rows_aligned(p.residual, p.residual_stride, size, 16);
-  a.w_vec = (uintptr_t)p.weight % 16 == 0;
-  a.h_vec = rows_aligned(p.h, p.h_stride, size, 16);
-  a.q_vec = rows_aligned(p.q, p.q_stride, 1, 16 / size);
+  // Every tensor's rows start on whole vectors (16 bytes; one byte a value of q).
+  const bool aligned = rows_aligned(p.x, p.x_stride, size, 16) && rows_aligned(p.q, p.q_stride, 1, 16 / size) &&
+              (!norm || (uintptr_t)p.weight % 16 == 0) &&
+              (!res || (rows_aligned(p.residual, p.residual_stride, size, 16) &&
+                        rows_aligned(p.h, p.h_stride, size, 16)));
   const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (p.dtype) {
     case TMLA_DTYPE_BF16:
-      e = norm ? run<__nv_bfloat16, true>(a, pdl, s) : run<__nv_bfloat16, false>(a, pdl, s);
+      e = norm ? run<__nv_bfloat16, true>(a, aligned, pdl, s) : run<__nv_bfloat16, false>(a, aligned, pdl, s);
       break;
     case TMLA_DTYPE_FP16:
-      e = norm ? run<__half, true>(a, pdl, s) : run<__half, false>(a, pdl, s);
+      e = norm ? run<__half, true>(a, aligned, pdl, s) : run<__half, false>(a, aligned, pdl, s);
       break;
     default:
-      e = norm ? run<float, true>(a, pdl, s) : run<float, false>(a, pdl, s);
+      e = norm ? run<float, true>(a, aligned, pdl, s) : run<float, false>(a, aligned, pdl, s);
       break;
   }
   if (e == cudaSuccess) e = cudaGetLastError();
