@@ -404,7 +404,14 @@ int tmla_rms_norm_int8(const TmlaInt8RowsParams* p, void* stream);
 
 /* y[i, j] = x_scale[i] * w_scale[j] * sum_c x[i, c] w[j, c], the sum exact in int32 (k at most
    TMLA_LINEAR_INT8_MAX_K, the longest whose sum of (-128)^2 terms fits), one rounding to dtype
-   at the end (fp32 products of the sum and the scales).  Any m, n >= 0 and k >= 1. */
+   at the end (fp32 products of the sum and the scales).  Any m, n from 0 to 2^30 and k >= 1.  Rows of x and
+   w that start on 16-byte boundaries (as tmla_quantize_int8 callers lay them out with strides
+   that are multiples of 16) run on the tcgen05 kernel, others on a CUDA-core kernel with the
+   same results.  No workspace: calls may overlap freely.  With TMLA_LAYER_FLAG_PDL the weight
+   loads may overlap the preceding kernel, which must not write w.  Every pipeline wait gives up
+   after wait_ns: the call then sets TMLA_STATUS_TIMEOUT in *status and leaves the output tiles
+   that it could not finish unwritten (TMLA_LINEAR_FLAG_TEST_STALL, for tests of that path only,
+   makes the first CTA skip its first loads). */
 #define TMLA_LINEAR_INT8_MAX_K 131071
 typedef struct TmlaLinearInt8Params {
   const void* x;                   /* int8 [m, k] */
@@ -418,6 +425,8 @@ typedef struct TmlaLinearInt8Params {
   int32_t m, n, k;
   int32_t dtype;                   /* TMLA_DTYPE_* of y */
   int32_t flags;                   /* TMLA_LAYER_FLAG_* */
+  int32_t* status;                 /* optional device status word (TMLA_STATUS_TIMEOUT) */
+  int64_t wait_ns;                 /* limit of each pipeline wait (<= 0: 2 s) */
 } TmlaLinearInt8Params;
 int tmla_linear_int8(const TmlaLinearInt8Params* p, void* stream);
 

@@ -399,3 +399,35 @@ def test_int8_operators_compile_without_a_graph_break(device):
     wq, ws = layer_ops.quantize_int8(torch.randn(70, 200, generator=g, device=device))
     for got, want in zip(torch.compile(f, fullgraph=True, backend="aot_eager")(x, r, w, wq, ws), f(x, r, w, wq, ws)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,n,k", [(16, 2112, 7168), (300, 700, 1024), (40, 130, 100)])
+def test_a_timed_out_wait_returns_cleanly(device, m, n, k):
+    """A bounded wait that runs out (the test-only stall: the first CTA never loads its first
+    stage) sets TMLA_STATUS_TIMEOUT and the kernel returns; the tiles of the other CTAs are right,
+    the stalled one's are left unwritten, and the next call is exact."""
+    import ctypes
+
+    from triton_mla import _lib
+    from triton_mla.kernel import _status_word
+
+    g = _gen(device, 11)
+    xq, wq = _int8(m, k, g, device), _int8(n, k, g, device)
+    xs, ws = torch.rand(m, generator=g, device=device), torch.rand(n, generator=g, device=device)
+    y = torch.full((m, n), float("nan"), device=device)
+    p = _lib.TmlaLinearInt8Params(xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0), ws.data_ptr(),
+                                  y.data_ptr(), n, m, n, k, _lib.DTYPE_FP32, _lib.LINEAR_FLAG_TEST_STALL,
+                                  _status_word(device).data_ptr(), 20_000_000)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    read_status(device)
+    assert _lib.load().tmla_linear_int8(ctypes.byref(p), stream) == 0
+    torch.cuda.synchronize()
+    assert read_status(device) == _lib.STATUS_TIMEOUT
+    ref = (xq.double() @ wq.double().T) * xs.double()[:, None] * ws.double()
+    missing = torch.isnan(y)
+    assert bool(missing[0, 0]) and bool(((y.double() - ref).abs()[~missing] <= ref.abs()[~missing] * 4 * U).all())
+    p.flags = 0
+    assert _lib.load().tmla_linear_int8(ctypes.byref(p), stream) == 0
+    torch.cuda.synchronize()
+    assert read_status(device) == 0
+    _compare_linear(y, xq, xs, wq, ws)

@@ -76,6 +76,8 @@ def _linear(**kw):
     (dict(x_stride=63), _lib.ERR_INVALID_ARG),
     (dict(w_stride=63), _lib.ERR_INVALID_ARG),
     (dict(y_stride=7), _lib.ERR_INVALID_ARG),
+    (dict(m=(1 << 30) + 1), _lib.ERR_UNSUPPORTED),
+    (dict(n=(1 << 30) + 1, y_stride=1 << 31), _lib.ERR_UNSUPPORTED),
     (dict(k=_lib.LINEAR_INT8_MAX_K + 1, x_stride=1 << 20, w_stride=1 << 20), _lib.ERR_UNSUPPORTED),
 ])
 def test_linear_int8_checks_its_arguments_before_any_launch(kw, code):
@@ -111,5 +113,5 @@ def test_int8_operators_have_meta_kernels():
     assert q.stride() == (1008, 1) and h.shape == x.shape and h.dtype == x.dtype
     assert ops.rms_norm_int8(x, w, 1e-6, None, None, False)[2].numel() == 0
     wq = torch.empty(70, 1001, dtype=torch.int8, device="meta")
-    y = ops.linear_int8(q, scale, wq, torch.empty(70, device="meta"), torch.float16, False)
+    y = ops.linear_int8(q, scale, wq, torch.empty(70, device="meta"), torch.float16, False, None)
     assert y.shape == (5, 70) and y.dtype == torch.float16

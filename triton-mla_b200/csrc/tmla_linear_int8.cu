@@ -1,11 +1,390 @@
 // int8 projections: y[i, j] = x_scale[i] w_scale[j] sum_c x[i, c] w[j, c], both operands int8 with
 // unit stride along c.  The sum is exact in int32 for k <= 131071 (|sum| <= k 2^14 < 2^31), so
 // neither the order of the terms nor the way k is cut changes the result.
+//
+// tcgen05 kernel (int8_kernel).  The weight rows (output channels) are the MMA's M and the tokens its
+// N, whatever their numbers: D[channel][token] then has one channel per TMEM lane, so that a
+// warp of the epilogue writes 32 neighbouring channels of a token at once, straight to y, and
+// one token or an odd n costs a predicate.  One instantiation serves all sizes; the token tile
+// N is an argument.
+//   kGroup = 1: one CTA per tile of 128 channels.
+//   kGroup = 2: a CTA pair per tile of 256 channels (cta_group::2): each CTA holds its 128 weight
+//     rows and half of the tokens, which halves what an MMA reads of the token operand.
+//   splits > 1: the CTAs (or pairs) of a cluster each take a part of k for the same tile.  Each
+//     accumulates in its own TMEM; then CTA s of the cluster adds up the token columns s of all
+//     through distributed shared memory and writes them.  No workspace, no counters, no atomics.
+// Per CTA (192 threads): warp 0 loads k-steps of 128 columns (128-byte swizzled boxes of w and x) by
+// TMA into a ring of stages; warp 1 issues the MMAs (the pair's even CTA for both); warps 2-5
+// are the epilogue, one thread per channel.  Unsplit CTAs are persistent, with two
+// accumulators, so that a tile's epilogue runs under the next tile's MMAs.
+//
+// Every wait is bounded (2 s by default): on expiry the kernel sets TMLA_STATUS_TIMEOUT, stops,
+// drains the copies and MMAs that it issued, leaves the tiles that it could not finish unwritten,
+// frees TMEM and returns.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "tmla_common.cuh"
 #include "tmla_ptx.cuh"
 
 namespace tmla {
+namespace sm100 {
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+}
 namespace linear_int8 {
+
+using namespace ptx;
+
+constexpr int kRows = 128;                 // weight rows per CTA (TMEM lanes)
+constexpr int kBoxK = 128;                 // columns per k-step: one swizzled 128-byte row
+constexpr int kWBytes = kRows * kBoxK;     // weight bytes of a stage
+constexpr int kMaxTok = 256;               // tokens per tile (MMA N)
+constexpr int kMaxSplits = 8;              // CTAs of a portable cluster
+constexpr int kMaxStages = 12;
+constexpr int kThreads = 192, kEpiThreads = 128;
+constexpr int kMaxRows = 1 << 30;          // tokens and channels: row numbers past a tile's end stay in int
+constexpr uint32_t kSmemMax = 227 * 1024;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+// After the ring: barriers full / empty per stage, accumulator full / empty (two), "MMAs done"; the TMEM
+// address, the abort flag, the gave-up flags of the cluster's CTAs, the epilogue's verdicts; the
+// token scales of two tiles.
+constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarAccFull = 2 * kMaxStages, kBarAccEmpty = kBarAccFull + 2,
+              kBarMmaDone = kBarAccEmpty + 2, kNumBars = kBarMmaDone + 1;
+constexpr uint32_t kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4, kOffPoison = kOffAbort + 4,
+                   kOffVerdict = kOffPoison + 4 * kMaxSplits, kOffScales = (kOffVerdict + 8 + 15) / 16 * 16,
+                   kTailBytes = kOffScales + 2 * kMaxTok * 4;
+
+struct Args {
+  int m, n;
+  int tok, splits;          // tokens per tile, parts of k
+  int n_tiles, t_tiles;     // tiles of channels and of tokens
+  int k_steps;
+  int stages, stage_bytes, x_bytes;  // x_bytes: this CTA's token rows of a stage
+  int acc_cols, tmem_cols;  // TMEM columns of an accumulator, and allocated
+  int band;                 // token tiles walked together (see tile_of)
+  const float* x_scale;
+  const float* w_scale;
+  void* y;
+  int64_t y_stride;
+  int* status;
+  unsigned long long wait_ns;
+  int stall;                // test only: the first CTA never loads its first stage
+};
+
+struct Waiter {
+  volatile int* abort_flag;
+  int* status;
+  uint64_t limit_ns;
+  __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) const {
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+      if (mbar_try_wait_cluster(bar, parity)) return true;
+      if ((i & 63) == 63) {
+        if (*abort_flag) return false;
+        const uint64_t now = globaltimer();
+        if (t0 == 0) {
+          t0 = now;
+        } else if (now - t0 > limit_ns) {
+          *abort_flag = 1;
+          if (status) atomicOr(status, TMLA_STATUS_TIMEOUT);
+          return false;
+        }
+      }
+    }
+  }
+};
+__device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait_cluster(bar, parity) && globaltimer() - t0 < limit_ns) {
+  }
+}
+
+// Tile number i as (channel tile, token tile).  Tiles that run at the same time are neighbours in bands
+// of `band` token tiles x all channel tiles, so that both operands are re-read from L2.
+__device__ __forceinline__ void tile_of(const Args& a, int i, int& tn, int& tt) {
+  const int per = a.band * a.n_tiles;
+  const int b = i / per, r = i - b * per;
+  const int rest = a.t_tiles - b * a.band, width = rest < a.band ? rest : a.band;
+  tn = r / width;
+  tt = b * a.band + (r - tn * width);
+}
+
+__device__ __forceinline__ void put(float v, float* y) { *y = v; }
+__device__ __forceinline__ void put(float v, __nv_bfloat16* y) { *y = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(float v, __half* y) { *y = __float2half_rn(v); }
+
+// Columns [c0, c0 + kCols) of a tile for this thread's channel: scaled, rounded and written.
+template <typename T, int kCols>
+__device__ __forceinline__ void write_columns(const Args& a, const uint32_t (&acc)[kCols], const float* scales, int c0,
+                                              int token0, T* y_channel, float w_scale, bool live) {
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    const int token = token0 + c0 + j;
+    const float v = (float)(int)acc[j] * scales[c0 + j] * w_scale;
+    if (live && token < a.m) put(v, y_channel + (int64_t)token * a.y_stride);
+  }
+}
+
+template <typename T, int kGroup>
+__global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ CUtensorMap tm_w,
+                                                        const __grid_constant__ CUtensorMap tm_x, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t tail = base + (uint32_t)(a.stages * a.stage_bytes);
+  uint8_t* tail_ptr = smem_raw + (tail - raw);
+  auto bar = [&](int i) { return tail + 8u * (uint32_t)i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_ptr + kOffAbort);
+  volatile int* poison = reinterpret_cast<volatile int*>(tail_ptr + kOffPoison);
+  volatile int* verdict = reinterpret_cast<volatile int*>(tail_ptr + kOffVerdict);
+  float* scales = reinterpret_cast<float*>(tail_ptr + kOffScales);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cluster_size = kGroup * a.splits;
+  const int rank = cluster_size > 1 ? (int)cluster_ctarank() : 0;
+  const int half = rank % kGroup, split = rank / kGroup;
+  const bool leader = half == 0;
+  const int cluster = (int)blockIdx.x / cluster_size, clusters = (int)gridDim.x / cluster_size;
+  const int tiles = a.n_tiles * a.t_tiles;
+  const int ks0 = (int)((long long)split * a.k_steps / a.splits);
+  const int ks1 = (int)((long long)(split + 1) * a.k_steps / a.splits);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < a.stages; ++s) {
+      mbar_init(bar(kBarFull + s), 1);
+      mbar_init(bar(kBarEmpty + s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(kBarAccFull + b), 1);
+      mbar_init(bar(kBarAccEmpty + b), kGroup * (kEpiThreads / 32));
+    }
+    mbar_init(bar(kBarMmaDone), 1);
+    *abort_flag = 0;
+    for (int i = 0; i < kMaxSplits; ++i) poison[i] = 0;
+    fence_mbar_init();
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  if (warp == 1) {
+    tmem_alloc_g<kGroup>(tail + kOffTmem, (uint32_t)a.tmem_cols);
+    tmem_relinquish_g<kGroup>();
+  }
+  tc_fence_before();
+  if (cluster_size > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kOffTmem);
+  const Waiter waiter{abort_flag, a.status, a.wait_ns};
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const bool stalled = a.stall && blockIdx.x == 0;
+      // A weight row is used by one token tile only, or again by the next ones.
+      const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
+      const uint64_t pol_x = policy_evict_last();
+      const uint32_t tx = (uint32_t)(kGroup * (kWBytes + a.x_bytes));
+      const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
+      auto load_w = [&](int s, int ks, int tn) {
+        const uint32_t st = base + (uint32_t)(s * a.stage_bytes), full = pair_bar + 8u * (uint32_t)(kBarFull + s);
+        const int row = (tn * kGroup + half) * kRows;
+        if constexpr (kGroup == 2)
+          tma_load_2d_pair(st, &tm_w, full, ks * kBoxK, row, pol_w);
+        else
+          tma_load_2d(st, &tm_w, full, ks * kBoxK, row, pol_w);
+      };
+      auto load_x = [&](int s, int ks, int tt) {
+        const uint32_t st = base + (uint32_t)(s * a.stage_bytes) + kWBytes,
+                       full = pair_bar + 8u * (uint32_t)(kBarFull + s);
+        const int row = tt * a.tok + half * (a.tok / kGroup);
+        if constexpr (kGroup == 2)
+          tma_load_2d_pair(st, &tm_x, full, ks * kBoxK, row, pol_x);
+        else
+          tma_load_2d(st, &tm_x, full, ks * kBoxK, row, pol_x);
+      };
+      // The weight boxes of the first stages do not depend on the kernel before (a programmatic
+      // launch): they are requested before it has completed.
+      int tn, tt, early = 0;
+      tile_of(a, cluster, tn, tt);
+      const int pre = ks1 - ks0 < a.stages ? ks1 - ks0 : a.stages;
+      early = pre < 2 ? pre : 2;
+      if (!stalled) {
+        for (int s = 0; s < early; ++s) {
+          if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx);
+          load_w(s, ks0 + s, tn);
+        }
+      }
+      griddep_wait();
+      griddep_launch_dependents();
+      long long i = 0;  // k-steps loaded so far (ring position)
+      bool ok = true;
+      for (int t = cluster; t < tiles && ok; t += clusters) {
+        tile_of(a, t, tn, tt);
+        for (int ks = ks0; ks < ks1; ++ks, ++i) {
+          const int s = (int)(i % a.stages);
+          const uint32_t round = (uint32_t)(i / a.stages);
+          if (round > 0) ok = waiter.wait(bar(kBarEmpty + s), (round - 1) & 1);
+          if (!ok) break;
+          if (stalled && i == 0) continue;
+          if (i >= early || stalled) {
+            if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx);
+            load_w(s, ks, tn);
+          }
+          load_x(s, ks, tt);
+        }
+      }
+      if (!ok && leader) {
+        // Let the copies in flight land before the CTA can exit.
+        for (long long j = i > a.stages ? i - a.stages : 0; j < i; ++j)
+          drain_wait(bar(kBarFull + (int)(j % a.stages)), (uint32_t)(j / a.stages) & 1, a.wait_ns);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      const uint32_t idesc = idesc_i8(kRows * kGroup, (uint32_t)a.tok);
+      const uint16_t mask = (uint16_t)(3u << (rank - half));
+      long long i = 0;
+      int iter = 0;
+      bool ok = true, issued = false;
+      for (int t = cluster; t < tiles && ok; t += clusters, ++iter) {
+        const int buf = iter & 1;
+        if (iter >= 2) ok = waiter.wait(bar(kBarAccEmpty + buf), (uint32_t)((iter >> 1) - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(buf * a.acc_cols);
+        for (int ks = ks0; ks < ks1; ++ks, ++i) {
+          const int s = (int)(i % a.stages);
+          ok = waiter.wait(bar(kBarFull + s), (uint32_t)(i / a.stages) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t st = base + (uint32_t)(s * a.stage_bytes);
+          const uint64_t adesc = smem_desc(st, 16, 1024, kSwizzle128B);
+          const uint64_t bdesc = smem_desc(st + kWBytes, 16, 1024, kSwizzle128B);
+#pragma unroll
+          for (int kk = 0; kk < kBoxK / 32; ++kk)  // 32 columns are 32 bytes along the swizzled row
+            mma_i8<kGroup>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, (ks > ks0 || kk > 0) ? 1u : 0u);
+          issued = true;
+          mma_commit_g<kGroup>(bar(kBarEmpty + s), mask);
+        }
+        if (!ok) break;
+        mma_commit_g<kGroup>(bar(kBarAccFull + buf), mask);
+      }
+      if (!ok && issued) {
+        mma_commit_g<kGroup>(bar(kBarMmaDone), (uint16_t)(1u << rank));
+        drain_wait(bar(kBarMmaDone), 0, a.wait_ns);
+      }
+    }
+    __syncwarp();
+  } else {
+    // Epilogue: thread `row` owns channel (TMEM lane) row of this CTA's 128.
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    griddep_wait();
+    int iter = 0;
+    bool gave_up = false;
+    for (int t = cluster; t < tiles && !gave_up; t += clusters, ++iter) {
+      int tn, tt;
+      tile_of(a, t, tn, tt);
+      const int buf = iter & 1;
+      const int channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
+      const bool live = channel < a.n;
+      const float w_scale = live ? a.w_scale[channel] : 0.f;
+      float* sc = scales + buf * kMaxTok;
+      for (int c = row; c < a.tok; c += kEpiThreads) sc[c] = token0 + c < a.m ? a.x_scale[token0 + c] : 0.f;
+      // One thread waits and the verdict is shared, so that all leave together.  Slot `buf` of verdict
+      // and scales is rewritten two tiles on, after everyone has passed the barrier between.
+      if (row == 0) verdict[buf] = waiter.wait(bar(kBarAccFull + buf), (uint32_t)(iter >> 1) & 1) ? 1 : 0;
+      named_sync(1, kEpiThreads);
+      gave_up = !verdict[buf];
+      if (gave_up || a.splits > 1) break;
+      tc_fence_after();
+      T* y = static_cast<T*>(a.y) + channel;
+      const uint32_t acc = lanes + (uint32_t)(buf * a.acc_cols);
+      for (int c = 0; c < a.tok; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(acc + (uint32_t)c, r);
+        tc_wait_ld();
+        write_columns<T, 16>(a, r, sc, c, token0, y, w_scale, live);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kGroup == 2)
+          mbar_arrive_cluster(map_to_rank(bar(kBarAccEmpty + buf), (uint32_t)(rank - half)));
+        else
+          mbar_arrive(bar(kBarAccEmpty + buf));
+      }
+    }
+    if (a.splits > 1 && gave_up && row == 0) {
+      for (int r = 0; r < cluster_size; ++r) st_cluster_u1(map_to_rank(tail + kOffPoison, (uint32_t)r) + 4u * split, 1u);
+    }
+    __syncwarp();
+  }
+
+  if (a.splits > 1) {
+    // One tile per cluster.  Every CTA's MMAs have read their ring, which now takes the parts of the
+    // columns that this CTA adds up: groups of 4 token columns, [part][group][channel] x 16 bytes.
+    cluster_sync();
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int groups = a.tok / 4, per = (groups + a.splits - 1) / a.splits;
+    const bool mine_ok = *abort_flag == 0;
+    if (warp >= 2 && mine_ok) {
+      tc_fence_after();
+      for (int c = 0; c < a.tok; c += 16) {
+        uint32_t r[16];
+        tmem_ld16(acc + (uint32_t)c, r);
+        tc_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int g = c / 4 + j, owner = g / per;
+          if (owner == split) continue;
+          const int part = split < owner ? split : split - 1;
+          const uint32_t at = base + (uint32_t)(((part * per + g - owner * per) * kRows + row) * 16);
+          st_cluster_u4(map_to_rank(at, (uint32_t)(owner * kGroup + half)), r[4 * j], r[4 * j + 1], r[4 * j + 2],
+                        r[4 * j + 3]);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    bool ok = mine_ok;
+    for (int i = 0; i < a.splits; ++i) ok = ok && poison[i] == 0;
+    if (warp >= 2 && ok) {
+      int tn, tt;
+      tile_of(a, cluster, tn, tt);
+      const int channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
+      const bool live = channel < a.n;
+      const float w_scale = live ? a.w_scale[channel] : 0.f;
+      T* y = static_cast<T*>(a.y) + channel;
+      const uint8_t* parts = smem_raw + (base - raw) + (size_t)row * 16;
+      for (int g = split * per; g < groups && g < (split + 1) * per; ++g) {
+        uint32_t r[4];
+        tmem_ld4(acc + (uint32_t)(4 * g), r);
+        tc_wait_ld();
+        for (int p = 0; p < a.splits - 1; ++p) {
+          const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + g - split * per) * kRows * 16);
+          r[0] += v.x, r[1] += v.y, r[2] += v.z, r[3] += v.w;
+        }
+        write_columns<T, 4>(a, r, scales, 4 * g, token0, y, w_scale, live);
+      }
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  if (cluster_size > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_g<kGroup>(tmem, (uint32_t)a.tmem_cols);
+  }
+}
 
 // ---------------------------------------------------------------------------- CUDA-core kernel
 // Rows of any alignment.  A block computes 64 tokens x 64 channels, 4 x 4 per thread, from 64
@@ -23,10 +402,6 @@ struct GenericArgs {
   int64_t y_stride;
   int m, n, k;
 };
-
-__device__ __forceinline__ void put(float v, float* y) { *y = v; }
-__device__ __forceinline__ void put(float v, __nv_bfloat16* y) { *y = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(float v, __half* y) { *y = __float2half_rn(v); }
 
 // Columns [k0, k0 + 64) of rows [r0, r0 + 64), zeros outside the matrix.
 __device__ __forceinline__ void stage(int (&dst)[kTile][kWords + 1], const int8_t* src, int64_t stride, int r0,
@@ -93,22 +468,141 @@ cudaError_t launch_generic(const GenericArgs& a, bool pdl, cudaStream_t stream) 
   return cudaLaunchKernelEx(&cfg, generic_kernel<T>, a);
 }
 
+// ---------------------------------------------------------------------------- host side
+struct Plan {
+  int group, tok, splits, stages;
+};
+
+int sm_count() {
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return -1;
+  return v;
+}
+
+Plan make_plan(int m, int n, int k, int sms) {
+  Plan p;
+  const int k_steps = (k + kBoxK - 1) / kBoxK;
+  p.group = m <= 128 ? 1 : 2;
+  p.tok = p.group == 1 ? (m <= 64 ? (m + 15) / 16 * 16 : (m + 31) / 32 * 32) : 256;
+  p.splits = 1;
+  const int n_tiles = (n + kRows * p.group - 1) / (kRows * p.group), t_tiles = (m + p.tok - 1) / p.tok;
+  while (p.splits < kMaxSplits / p.group && p.splits * 2 <= k_steps && p.group * n_tiles * t_tiles * p.splits * 2 <= 2 * sms) p.splits *= 2;
+  const int stage = kWBytes + p.tok / p.group * kBoxK;
+  const int budget = p.group * n_tiles * t_tiles * p.splits > sms && p.splits > 1 ? 96 * 1024 : 200 * 1024;
+  p.stages = budget / stage;
+  if (p.stages > kMaxStages) p.stages = kMaxStages;
+  return p;
+}
+
+// A matrix of int8 rows as a map of boxes of `rows` rows x 128 swizzled bytes; outside it reads zeros.
+int encode(CUtensorMap* map, const void* base, int k, int rows, int64_t stride, int box_rows) {
+  auto fn = sm100::encode_fn();
+  if (!fn) return TMLA_ERR_CUDA;
+  cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)stride};
+  cuuint32_t box[2] = {kBoxK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : TMLA_ERR_MISALIGNED;
+}
+
+template <typename T, int kGroup>
+cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const Args& a, int clusters, size_t smem, bool pdl,
+                      cudaStream_t stream) {
+  cudaError_t e =
+      cudaFuncSetAttribute(int8_kernel<T, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  const int size = kGroup * a.splits;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)size;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)(clusters * size));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, int8_kernel<T, kGroup>, tw, tx, a);
+}
+
+template <typename T>
+cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensorMap& tw, const CUtensorMap& tx, int sms,
+                   cudaStream_t stream) {
+  Args a;
+  a.m = p.m;
+  a.n = p.n;
+  a.tok = pl.tok;
+  a.splits = pl.splits;
+  a.n_tiles = (p.n + kRows * pl.group - 1) / (kRows * pl.group);
+  a.t_tiles = (p.m + pl.tok - 1) / pl.tok;
+  a.k_steps = (p.k + kBoxK - 1) / kBoxK;
+  a.x_bytes = pl.tok / pl.group * kBoxK;
+  a.stages = pl.stages;
+  a.stage_bytes = kWBytes + a.x_bytes;
+  const int tiles = a.n_tiles * a.t_tiles;
+  const int resident = sms / pl.group;
+  const int clusters = pl.splits > 1 || tiles < resident ? tiles : resident;
+  a.acc_cols = (pl.tok + 31) / 32 * 32;
+  const int cols = a.acc_cols * (tiles > clusters ? 2 : 1);
+  for (a.tmem_cols = 32; a.tmem_cols < cols;) a.tmem_cols *= 2;
+  a.band = a.t_tiles < 8 ? a.t_tiles : 8;
+  a.x_scale = p.x_scale;
+  a.w_scale = p.w_scale;
+  a.y = p.y;
+  a.y_stride = p.y_stride;
+  a.status = p.status;
+  a.wait_ns = p.wait_ns > 0 ? (unsigned long long)p.wait_ns : kWaitNs;
+  a.stall = (p.flags & TMLA_LINEAR_FLAG_TEST_STALL) ? 1 : 0;
+  // What the kernel takes for granted: a ring, at least one k-step per part, the parts of the columns that a
+  // CTA adds up fit into the ring.
+  const int per = (pl.tok / 4 + pl.splits - 1) / pl.splits;
+  if (a.stages < 1 || pl.splits > a.k_steps || pl.splits * pl.group > kMaxSplits || pl.tok > kMaxTok ||
+      pl.tok % (16 * pl.group) || (long long)(pl.splits - 1) * per * kRows * 16 > (long long)a.stages * a.stage_bytes)
+    return cudaErrorInvalidValue;
+  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + kTailBytes;
+  const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
+  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, a, clusters, smem, pdl, stream)
+                       : launch_tc<T, 2>(tw, tx, a, clusters, smem, pdl, stream);
+}
+
 int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
   if (p.m < 0 || p.n < 0 || p.k < 1) return TMLA_ERR_INVALID_ARG;
   if (p.dtype != TMLA_DTYPE_BF16 && p.dtype != TMLA_DTYPE_FP16 && p.dtype != TMLA_DTYPE_FP32)
     return TMLA_ERR_INVALID_ARG;
-  if (p.k > TMLA_LINEAR_INT8_MAX_K) return TMLA_ERR_UNSUPPORTED;
+  if (p.k > TMLA_LINEAR_INT8_MAX_K || p.m > kMaxRows || p.n > kMaxRows) return TMLA_ERR_UNSUPPORTED;
   if (p.m == 0 || p.n == 0) return TMLA_OK;
   if (!p.x || !p.x_scale || !p.w || !p.w_scale || !p.y) return TMLA_ERR_INVALID_ARG;
   if (p.x_stride < p.k || p.w_stride < p.k || p.y_stride < p.n) return TMLA_ERR_INVALID_ARG;
   const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
-  const GenericArgs a{static_cast<const int8_t*>(p.x), p.x_stride, p.x_scale, static_cast<const int8_t*>(p.w),
-                      p.w_stride, p.w_scale, p.y, p.y_stride, p.m, p.n, p.k};
   cudaError_t e;
-  switch (p.dtype) {
-    case TMLA_DTYPE_BF16: e = launch_generic<__nv_bfloat16>(a, pdl, stream); break;
-    case TMLA_DTYPE_FP16: e = launch_generic<__half>(a, pdl, stream); break;
-    default: e = launch_generic<float>(a, pdl, stream); break;
+  if ((((uintptr_t)p.x | (uintptr_t)p.w) % 16 || p.x_stride % 16 || p.w_stride % 16)) {
+    const GenericArgs a{static_cast<const int8_t*>(p.x), p.x_stride, p.x_scale, static_cast<const int8_t*>(p.w),
+                        p.w_stride, p.w_scale, p.y, p.y_stride, p.m, p.n, p.k};
+    switch (p.dtype) {
+      case TMLA_DTYPE_BF16: e = launch_generic<__nv_bfloat16>(a, pdl, stream); break;
+      case TMLA_DTYPE_FP16: e = launch_generic<__half>(a, pdl, stream); break;
+      default: e = launch_generic<float>(a, pdl, stream); break;
+    }
+  } else {
+    const int sms = sm_count();
+    if (sms < 1) return record_cuda_error(cudaGetLastError());
+    const Plan pl = make_plan(p.m, p.n, p.k, sms);
+    CUtensorMap tw, tx;
+    int rc = encode(&tw, p.w, p.k, p.n, p.w_stride, kRows);
+    if (!rc) rc = encode(&tx, p.x, p.k, p.m, p.x_stride, pl.tok / pl.group);
+    if (rc) return rc;
+    switch (p.dtype) {
+      case TMLA_DTYPE_BF16: e = launch<__nv_bfloat16>(p, pl, tw, tx, sms, stream); break;
+      case TMLA_DTYPE_FP16: e = launch<__half>(p, pl, tw, tx, sms, stream); break;
+      default: e = launch<float>(p, pl, tw, tx, sms, stream); break;
+    }
   }
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? TMLA_OK : record_cuda_error(e);

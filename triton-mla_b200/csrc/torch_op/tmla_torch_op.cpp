@@ -120,8 +120,8 @@ void check_rows(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.dim() == 2 && (t.size(1) == 0 || t.stride(1) == 1), "triton_mla: ", what,
               " must be a matrix with unit inner stride");
 }
-// A one-row matrix may carry any row stride; the library wants at least the row's length.
-int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+// A one-row matrix may carry any row stride, which nothing reads: one that breaks no alignment.
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
 
 void check_rc(int rc, const char* what) {
   TORCH_CHECK(rc == TMLA_OK, what, " failed: ", tmla_error_string(rc), " ",
@@ -205,7 +205,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_meta(const at::Tens
 }
 
 at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w,
-                            const at::Tensor& w_scale, at::ScalarType out_dtype, bool overlap) {
+                            const at::Tensor& w_scale, at::ScalarType out_dtype, bool overlap,
+                            const std::optional<at::Tensor>& status) {
   check_rows(x, "x_q");
   check_rows(w, "w_q");
   TORCH_CHECK(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar && x.size(1) == w.size(1) &&
@@ -233,12 +234,13 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
   p.n = (int32_t)w.size(0);
   p.k = (int32_t)x.size(1);
   p.dtype = dtype_code(out_dtype);
+  p.status = status.has_value() ? status->data_ptr<int32_t>() : nullptr;
   p.flags = overlap ? TMLA_LAYER_FLAG_PDL : 0;
   check_rc(tmla_linear_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), "tmla_linear_int8");
   return y;
 }
 at::Tensor linear_int8_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
-                            at::ScalarType out_dtype, bool) {
+                            at::ScalarType out_dtype, bool, const std::optional<at::Tensor>&) {
   return at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
 }
 
@@ -258,8 +260,8 @@ TORCH_LIBRARY(triton_mla, m) {
       "rms_norm_int8(Tensor x, Tensor weight, float eps, Tensor? residual, Tensor(a!)? residual_out, bool overlap) "
       "-> (Tensor, Tensor, Tensor)");
   m.def(
-      "linear_int8(Tensor x_q, Tensor x_scale, Tensor w_q, Tensor w_scale, ScalarType out_dtype, bool overlap) "
-      "-> Tensor");
+      "linear_int8(Tensor x_q, Tensor x_scale, Tensor w_q, Tensor w_scale, ScalarType out_dtype, bool overlap, "
+      "Tensor? status) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(triton_mla, CUDA, m) {

@@ -264,6 +264,8 @@ class TmlaLinearInt8Params(ctypes.Structure):
         ("k", ctypes.c_int32),
         ("dtype", ctypes.c_int32),
         ("flags", ctypes.c_int32),
+        ("status", ctypes.c_void_p),
+        ("wait_ns", ctypes.c_int64),
     ]
 
 

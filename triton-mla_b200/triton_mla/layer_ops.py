@@ -282,4 +282,5 @@ def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_s
     assert x_q.shape[1] <= _lib.LINEAR_INT8_MAX_K, "the int32 sum of a longer k can overflow"
     if out_dtype not in _DTYPE_CODES:
         raise TypeError(f"unsupported out_dtype {out_dtype}; use bfloat16, float16 or float32")
-    return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap)
+    status = None if torch.compiler.is_compiling() else _status_word(x_q.device)
+    return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap, status)
