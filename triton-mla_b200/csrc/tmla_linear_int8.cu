@@ -13,9 +13,9 @@
 //   splits > 1: the CTAs (or pairs) of a cluster each take a part of k for the same tile.  Each
 //     accumulates in its own TMEM; then CTA s of the cluster adds up the token columns s of all
 //     through distributed shared memory and writes them.  No workspace, no counters, no atomics.
-// Per CTA (192 threads): warp 0 loads k-steps of 128 columns (128-byte swizzled boxes of w and x) by
-// TMA into a ring of stages; warp 1 issues the MMAs (the pair's even CTA for both); warps 2-5
-// are the epilogue, one thread per channel.  Unsplit CTAs are persistent, with two
+// Per CTA (352 threads): warp 0 loads k-steps of 128 columns (128-byte swizzled boxes of w and x) by
+// TMA into a ring of stages; warp 1 issues the MMAs (the pair's even CTA for both); warps 2-9
+// are the epilogue; warp 10 stores what they stage.  Unsplit CTAs are persistent, with two
 // accumulators, so that a tile's epilogue runs under the next tile's MMAs.
 //
 // Every wait is bounded (2 s by default): on expiry the kernel sets TMLA_STATUS_TIMEOUT, stops,
@@ -41,19 +41,30 @@ constexpr int kWBytes = kRows * kBoxK;     // weight bytes of a stage
 constexpr int kMaxTok = 256;               // tokens per tile (MMA N)
 constexpr int kMaxSplits = 8;              // CTAs of a portable cluster
 constexpr int kMaxStages = 12;
-constexpr int kThreads = 192, kEpiThreads = 128;
+constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
+constexpr int kStoreWarp = 2 + kEpiWarps;
+constexpr int kThreads = 32 * (kStoreWarp + 1);
+// y leaves in chunks of 128 channels x 2 kBoxTok<T> tokens, staged in shared memory as boxes of 128 bytes
+// of channels x kBoxTok<T> tokens.
+constexpr uint32_t kChunkBytes = 16384;
+constexpr int kChunkBufs = 2;
+constexpr uint32_t kStagingBytes = kChunkBufs * kChunkBytes;
+template <typename T>
+constexpr int kBoxTok = (int)(kChunkBytes / (2 * kRows * sizeof(T)));  // 32 of 16 bits, 16 of fp32
+template <typename T>
+constexpr int kBoxChannels = (int)(128 / sizeof(T));
 constexpr int kMaxRows = 1 << 30;          // tokens and channels: row numbers past a tile's end stay in int
 constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-// After the ring: barriers full / empty per stage, accumulator full / empty (two), "MMAs done"; the TMEM
-// address, the abort flag, the gave-up flags of the cluster's CTAs, the epilogue's verdicts; the
-// token scales of two tiles.
+// After the ring and the staged chunks: barriers full / empty per stage, accumulator full / empty (two),
+// "MMAs done", chunk full / empty; the TMEM address, the abort flag, the gave-up flags of the
+// cluster's parts.
 constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarAccFull = 2 * kMaxStages, kBarAccEmpty = kBarAccFull + 2,
-              kBarMmaDone = kBarAccEmpty + 2, kNumBars = kBarMmaDone + 1;
+              kBarMmaDone = kBarAccEmpty + 2, kBarChunkFull = kBarMmaDone + 1, kBarChunkEmpty = kBarChunkFull + kChunkBufs,
+              kNumBars = kBarChunkEmpty + kChunkBufs;
 constexpr uint32_t kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4, kOffPoison = kOffAbort + 4,
-                   kOffVerdict = kOffPoison + 4 * kMaxSplits, kOffScales = (kOffVerdict + 8 + 15) / 16 * 16,
-                   kTailBytes = kOffScales + 2 * kMaxTok * 4;
+                   kTailBytes = kOffPoison + 4 * kMaxSplits;
 
 struct Args {
   int m, n;
@@ -62,6 +73,7 @@ struct Args {
   int k_steps;
   int stages, stage_bytes, x_bytes;  // x_bytes: this CTA's token rows of a stage
   int acc_cols, tmem_cols;  // TMEM columns of an accumulator, and allocated
+  int tma_store;            // y's rows start on 16-byte boundaries: TMA stores (else copied by the epilogue)
   int band;                 // token tiles walked together (see tile_of)
   const float* x_scale;
   const float* w_scale;
@@ -76,10 +88,13 @@ struct Waiter {
   volatile int* abort_flag;
   int* status;
   uint64_t limit_ns;
+  // kCluster: the arrivals come from threads of another CTA (acquire at cluster scope, which costs more
+  // than the loads and MMA completions of a stage should pay).
+  template <bool kCluster = false>
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) const {
     uint64_t t0 = 0;
     for (uint32_t i = 0;; ++i) {
-      if (mbar_try_wait_cluster(bar, parity)) return true;
+      if (kCluster ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
       if ((i & 63) == 63) {
         if (*abort_flag) return false;
         const uint64_t now = globaltimer();
@@ -93,10 +108,15 @@ struct Waiter {
       }
     }
   }
+  // The same for a converged warp, with one verdict.
+  template <bool kCluster = false>
+  __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity) const {
+    return __all_sync(0xffffffffu, wait<kCluster>(bar, parity));
+  }
 };
 __device__ __forceinline__ void drain_wait(uint32_t bar, uint32_t parity, uint64_t limit_ns) {
   const uint64_t t0 = globaltimer();
-  while (!mbar_try_wait_cluster(bar, parity) && globaltimer() - t0 < limit_ns) {
+  while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < limit_ns) {
   }
 }
 
@@ -114,33 +134,152 @@ __device__ __forceinline__ void put(float v, float* y) { *y = v; }
 __device__ __forceinline__ void put(float v, __nv_bfloat16* y) { *y = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void put(float v, __half* y) { *y = __float2half_rn(v); }
 
-// Columns [c0, c0 + kCols) of a tile for this thread's channel: scaled, rounded and written.
+// The scale of a token (of the last one for a row past the end, whose products are never written).
+__device__ __forceinline__ float token_scale(const Args& a, int token) { return a.x_scale[min(token, a.m - 1)]; }
+
+// kCols (a power of two) token columns from token0 on for this thread's channel: scaled, rounded and
+// written, by a converged warp.
 template <typename T, int kCols>
-__device__ __forceinline__ void write_columns(const Args& a, const uint32_t (&acc)[kCols], const float* scales, int c0,
-                                              int token0, T* y_channel, float w_scale, bool live) {
+__device__ __forceinline__ void write_columns(const Args& a, const uint32_t (&acc)[kCols], int token0, T* y_channel,
+                                              float w_scale, bool live) {
+  T* y = y_channel + (int64_t)token0 * a.y_stride;
+  const int tokens = live ? a.m - token0 : 0;
+  const float scale = token_scale(a, token0 + (int)(threadIdx.x % kCols));
 #pragma unroll
   for (int j = 0; j < kCols; ++j) {
-    const int token = token0 + c0 + j;
-    const float v = (float)(int)acc[j] * scales[c0 + j] * w_scale;
-    if (live && token < a.m) put(v, y_channel + (int64_t)token * a.y_stride);
+    const float v = (float)(int)acc[j] * __shfl_sync(0xffffffffu, scale, j) * w_scale;
+    if (j < tokens) put(v, y + j * a.y_stride);
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Past a wait for TMEM loads: their registers are read after it.
+template <int N>
+__device__ __forceinline__ void loaded(uint32_t (&r)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// A warp's share of a box of tokens: its 32 channels x half of the tokens, from `token` and `acc` on.
+// 16-bit y: 16 tokens.  The 16x256b loads leave the accumulator in the registers as 8 x 8 matrices of
+// channels x tokens, which stmatrix writes transposed into 128-byte swizzled rows of 64 channels.
+// fp32 y: 8 tokens, a thread's channel straight into rows of 32 channels.
+template <typename T>
+struct Share {
+  uint32_t r[16];
+  float s[4];
+  __device__ __forceinline__ void load(const Args& a, uint32_t acc, int token, int lane) {
+    tmem_ld16x256_x2(acc, *reinterpret_cast<uint32_t(*)[8]>(r));
+    tmem_ld16x256_x2(acc + (16u << 16), *reinterpret_cast<uint32_t(*)[8]>(r + 8));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = token_scale(a, token + 8 * (j >> 1) + 2 * (lane & 3) + (j & 1));
+  }
+  __device__ __forceinline__ void loaded() { linear_int8::loaded(r); }
+  // The channels whose scales a thread needs (of its warp's 32), and how many.
+  static constexpr int kScales = 4;
+  static __device__ __forceinline__ int channel(int j, int lane) { return 8 * j + (lane >> 2); }
+  __device__ __forceinline__ void put(uint32_t stage, const float (&ws)[kScales], int quarter, int sub,
+                                      int lane) const {
+    const T* t = nullptr;
+    const int mat = lane >> 3, mrow = lane & 7;
+    const uint32_t row =
+        stage + (uint32_t)((quarter >> 1) * kBoxTok<T> + 16 * sub + 8 * (mat >> 1) + mrow) * 128;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t* q = r + 8 * h + 4 * j;
+        v[2 * j] = pack2((float)(int)q[0] * s[2 * j] * ws[2 * h], (float)(int)q[1] * s[2 * j + 1] * ws[2 * h], t);
+        v[2 * j + 1] =
+            pack2((float)(int)q[2] * s[2 * j] * ws[2 * h + 1], (float)(int)q[3] * s[2 * j + 1] * ws[2 * h + 1], t);
+      }
+      const uint32_t chunk16 = (uint32_t)((quarter & 1) * 4 + h * 2 + (mat & 1));
+      stmatrix_x4_trans(row + ((chunk16 ^ (uint32_t)mrow) << 4), v[0], v[1], v[2], v[3]);
+    }
+  }
+};
+template <>
+struct Share<float> {
+  uint32_t r[8];
+  float s[8];
+  __device__ __forceinline__ void load(const Args& a, uint32_t acc, int token, int) {
+    tmem_ld8(acc, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] = token_scale(a, token + j);
+  }
+  __device__ __forceinline__ void loaded() { linear_int8::loaded(r); }
+  static constexpr int kScales = 1;
+  static __device__ __forceinline__ int channel(int, int lane) { return lane; }
+  __device__ __forceinline__ void put(uint32_t stage, const float (&ws)[kScales], int quarter, int sub,
+                                      int lane) const {
+    const uint32_t at = stage + (uint32_t)(quarter * kBoxTok<float> + 8 * sub) * 128 + (uint32_t)lane * 4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 128u * j), "f"((float)(int)r[j] * s[j] * ws[0]) : "memory");
+  }
+};
+
+// Row `i` of a staged chunk (128 channels) to y, of which `left` channels exist: for rows of y that TMA
+// cannot store to.  All 32 threads of a warp.
+template <typename T>
+__device__ __forceinline__ void copy_row(const uint8_t* chunk, int i, T* y, int left, int lane) {
+  const uint8_t* box = chunk + (i / kBoxTok<T>) * (kChunkBytes / 2) + (i % kBoxTok<T>) * 128;
+  constexpr int kBoxBytes = kBoxTok<T> * 128;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+      if (32 * b + lane < left) y[32 * b + lane] = *reinterpret_cast<const float*>(box + b * kBoxBytes + lane * 4);
+  } else {
+    // Word `lane` of each box holds channels 2 lane, 2 lane + 1 (and 64 on).
+    const int at = (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4;
+    uint32_t w[2];
+    w[0] = *reinterpret_cast<const uint32_t*>(box + at);
+    w[1] = *reinterpret_cast<const uint32_t*>(box + kBoxBytes + at);
+    const int odd = (int)(((uintptr_t)y >> 1) & 1);
+    uint16_t* out = reinterpret_cast<uint16_t*>(y);
+    if (odd) {
+      // Whole words of y hold channels 2 j + 1, 2 j + 2; the first channel is written alone.
+      const uint32_t next0 = __shfl_sync(0xffffffffu, lane == 0 ? w[1] : w[0], (lane + 1) & 31);
+      const uint32_t next1 = __shfl_sync(0xffffffffu, w[1], (lane + 1) & 31);
+      if (lane == 0 && left > 0) out[0] = (uint16_t)w[0];
+      w[0] = __byte_perm(w[0], next0, 0x5432);
+      w[1] = __byte_perm(w[1], next1, 0x5432);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int ch = 64 * b + 2 * lane + odd;
+      if (ch + 1 < left && ch + 1 < kRows)
+        *reinterpret_cast<uint32_t*>(out + ch) = w[b];
+      else if (ch < left && ch < kRows)
+        out[ch] = (uint16_t)w[b];
+    }
   }
 }
 
 template <typename T, int kGroup>
 __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ CUtensorMap tm_w,
-                                                        const __grid_constant__ CUtensorMap tm_x, const Args a) {
+                                                        const __grid_constant__ CUtensorMap tm_x,
+                                                        const __grid_constant__ CUtensorMap tm_y, const Args a) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  const uint32_t tail = base + (uint32_t)(a.stages * a.stage_bytes);
+  const uint32_t staging = base + (uint32_t)(a.stages * a.stage_bytes);
+  const uint32_t tail = staging + (a.splits == 1 ? kStagingBytes : 0);
   uint8_t* tail_ptr = smem_raw + (tail - raw);
   auto bar = [&](int i) { return tail + 8u * (uint32_t)i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_ptr + kOffAbort);
   volatile int* poison = reinterpret_cast<volatile int*>(tail_ptr + kOffPoison);
-  volatile int* verdict = reinterpret_cast<volatile int*>(tail_ptr + kOffVerdict);
-  float* scales = reinterpret_cast<float*>(tail_ptr + kOffScales);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cluster_size = kGroup * a.splits;
   const int rank = cluster_size > 1 ? (int)cluster_ctarank() : 0;
   const int half = rank % kGroup, split = rank / kGroup;
@@ -157,7 +296,11 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(kBarAccFull + b), 1);
-      mbar_init(bar(kBarAccEmpty + b), kGroup * (kEpiThreads / 32));
+      mbar_init(bar(kBarAccEmpty + b), kGroup * kEpiWarps);
+    }
+    for (int b = 0; b < kChunkBufs; ++b) {
+      mbar_init(bar(kBarChunkFull + b), kEpiWarps);
+      mbar_init(bar(kBarChunkEmpty + b), a.tma_store ? 1 : kEpiWarps);
     }
     mbar_init(bar(kBarMmaDone), 1);
     *abort_flag = 0;
@@ -180,147 +323,215 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   const Waiter waiter{abort_flag, a.status, a.wait_ns};
 
   if (warp == 0) {
-    if (lane == 0) {
-      const bool stalled = a.stall && blockIdx.x == 0;
-      // A weight row is used by one token tile only, or again by the next ones.
-      const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
-      const uint64_t pol_x = policy_evict_last();
-      const uint32_t tx = (uint32_t)(kGroup * (kWBytes + a.x_bytes));
-      const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
-      auto load_w = [&](int s, int ks, int tn) {
-        const uint32_t st = base + (uint32_t)(s * a.stage_bytes), full = pair_bar + 8u * (uint32_t)(kBarFull + s);
-        const int row = (tn * kGroup + half) * kRows;
-        if constexpr (kGroup == 2)
-          tma_load_2d_pair(st, &tm_w, full, ks * kBoxK, row, pol_w);
-        else
-          tma_load_2d(st, &tm_w, full, ks * kBoxK, row, pol_w);
-      };
-      auto load_x = [&](int s, int ks, int tt) {
-        const uint32_t st = base + (uint32_t)(s * a.stage_bytes) + kWBytes,
-                       full = pair_bar + 8u * (uint32_t)(kBarFull + s);
-        const int row = tt * a.tok + half * (a.tok / kGroup);
-        if constexpr (kGroup == 2)
-          tma_load_2d_pair(st, &tm_x, full, ks * kBoxK, row, pol_x);
-        else
-          tma_load_2d(st, &tm_x, full, ks * kBoxK, row, pol_x);
-      };
-      // The weight boxes of the first stages do not depend on the kernel before (a programmatic
-      // launch): they are requested before it has completed.
-      int tn, tt, early = 0;
-      tile_of(a, cluster, tn, tt);
-      const int pre = ks1 - ks0 < a.stages ? ks1 - ks0 : a.stages;
-      early = pre < 2 ? pre : 2;
-      if (!stalled) {
-        for (int s = 0; s < early; ++s) {
-          if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx);
-          load_w(s, ks0 + s, tn);
+    // The whole warp runs this (its operands stay warp-uniform); one thread issues.
+    const uint32_t elected = elect_one();
+    const bool stalled = a.stall && blockIdx.x == 0;
+    // A weight row is used by one token tile only, or again by the next ones.
+    const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
+    const uint64_t pol_x = policy_evict_last();
+    const uint32_t tx = (uint32_t)(kGroup * (kWBytes + a.x_bytes));
+    const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
+    auto load_w = [&](int s, int ks, int row) {
+      tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes), &tm_w, pair_bar + 8u * (uint32_t)(kBarFull + s),
+                          ks * kBoxK, row, pol_w, elected);
+    };
+    // The weight boxes of the first stages do not depend on the kernel before (a programmatic
+    // launch): they are requested before it has completed.
+    int tn, tt;
+    tile_of(a, cluster, tn, tt);
+    const int pre = ks1 - ks0 < a.stages ? ks1 - ks0 : a.stages, early = pre < 2 ? pre : 2;
+    for (int j = 0; j < early; ++j) {
+      if (stalled && j == 0) continue;
+      if (leader) mbar_arrive_expect_tx(bar(kBarFull + j), tx, elected);
+      load_w(j, ks0 + j, (tn * kGroup + half) * kRows);
+    }
+    griddep_wait();
+    griddep_launch_dependents();
+    int s = 0;           // ring position, and how often the ring has wrapped
+    uint32_t round = 0;
+    bool ok = true;
+    for (int t = cluster; t < tiles && ok; t += clusters) {
+      tile_of(a, t, tn, tt);
+      const int w_row = (tn * kGroup + half) * kRows, x_row = tt * a.tok + half * (a.tok / kGroup);
+      for (int ks = ks0; ks < ks1; ++ks) {
+        if (round > 0) ok = waiter.wait_warp(bar(kBarEmpty + s), (round - 1) & 1);
+        if (!ok) break;
+        if (round > 0 || s >= early) {
+          if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx, elected);
+          load_w(s, ks, w_row);
         }
+        if (!stalled || round > 0 || s > 0)
+          tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes) + kWBytes, &tm_x,
+                              pair_bar + 8u * (uint32_t)(kBarFull + s), ks * kBoxK, x_row, pol_x, elected);
+        if (++s == a.stages) s = 0, ++round;
       }
-      griddep_wait();
-      griddep_launch_dependents();
-      long long i = 0;  // k-steps loaded so far (ring position)
-      bool ok = true;
-      for (int t = cluster; t < tiles && ok; t += clusters) {
-        tile_of(a, t, tn, tt);
-        for (int ks = ks0; ks < ks1; ++ks, ++i) {
-          const int s = (int)(i % a.stages);
-          const uint32_t round = (uint32_t)(i / a.stages);
-          if (round > 0) ok = waiter.wait(bar(kBarEmpty + s), (round - 1) & 1);
-          if (!ok) break;
-          if (stalled && i == 0) continue;
-          if (i >= early || stalled) {
-            if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx);
-            load_w(s, ks, tn);
-          }
-          load_x(s, ks, tt);
-        }
-      }
-      if (!ok && leader) {
-        // Let the copies in flight land before the CTA can exit.
-        for (long long j = i > a.stages ? i - a.stages : 0; j < i; ++j)
-          drain_wait(bar(kBarFull + (int)(j % a.stages)), (uint32_t)(j / a.stages) & 1, a.wait_ns);
-      }
+    }
+    if (!ok && leader) {
+      // Let the copies in flight land before the CTA can exit.  (A wait gives up in a later round than
+      // the first, so every stage has been loaded.)
+      for (int j = 0; j < a.stages; ++j)
+        drain_wait(bar(kBarFull + j), (j < s ? round : round - 1) & 1, a.wait_ns);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    // The whole warp runs this (its operands stay warp-uniform); one thread issues.
+    if (leader) {
+      const uint32_t elected = elect_one();
       const uint32_t idesc = idesc_i8(kRows * kGroup, (uint32_t)a.tok);
       const uint16_t mask = (uint16_t)(3u << (rank - half));
-      long long i = 0;
-      int iter = 0;
+      int iter = 0, s = 0;
+      uint32_t phase = 0;  // parity of the ring's current round
       bool ok = true, issued = false;
       for (int t = cluster; t < tiles && ok; t += clusters, ++iter) {
         const int buf = iter & 1;
-        if (iter >= 2) ok = waiter.wait(bar(kBarAccEmpty + buf), (uint32_t)((iter >> 1) - 1) & 1);
+        if (iter >= 2) ok = waiter.wait_warp<(kGroup == 2)>(bar(kBarAccEmpty + buf), (uint32_t)((iter >> 1) - 1) & 1);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(buf * a.acc_cols);
-        for (int ks = ks0; ks < ks1; ++ks, ++i) {
-          const int s = (int)(i % a.stages);
-          ok = waiter.wait(bar(kBarFull + s), (uint32_t)(i / a.stages) & 1);
+        for (int ks = ks0; ks < ks1; ++ks) {
+          ok = waiter.wait_warp(bar(kBarFull + s), phase);
           if (!ok) break;
           tc_fence_after();
           const uint32_t st = base + (uint32_t)(s * a.stage_bytes);
-          const uint64_t adesc = smem_desc(st, 16, 1024, kSwizzle128B);
-          const uint64_t bdesc = smem_desc(st + kWBytes, 16, 1024, kSwizzle128B);
-#pragma unroll
-          for (int kk = 0; kk < kBoxK / 32; ++kk)  // 32 columns are 32 bytes along the swizzled row
-            mma_i8<kGroup>(d, adesc + 2 * kk, bdesc + 2 * kk, idesc, (ks > ks0 || kk > 0) ? 1u : 0u);
+          mma_i8_k128<kGroup>(d, smem_desc(st, 16, 1024, kSwizzle128B), smem_desc(st + kWBytes, 16, 1024, kSwizzle128B),
+                              idesc, ks > ks0 ? 1u : 0u, elected);
           issued = true;
-          mma_commit_g<kGroup>(bar(kBarEmpty + s), mask);
+          mma_commit_g<kGroup>(bar(kBarEmpty + s), mask, elected);
+          if (++s == a.stages) s = 0, phase ^= 1;
         }
         if (!ok) break;
-        mma_commit_g<kGroup>(bar(kBarAccFull + buf), mask);
+        mma_commit_g<kGroup>(bar(kBarAccFull + buf), mask, elected);
       }
       if (!ok && issued) {
-        mma_commit_g<kGroup>(bar(kBarMmaDone), (uint16_t)(1u << rank));
+        mma_commit_g<kGroup>(bar(kBarMmaDone), (uint16_t)(1u << rank), elected);
         drain_wait(bar(kBarMmaDone), 0, a.wait_ns);
       }
     }
     __syncwarp();
-  } else {
-    // Epilogue: thread `row` owns channel (TMEM lane) row of this CTA's 128.
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+  } else if (warp < kStoreWarp) {
+    // Epilogue: two warps per 32 channels (TMEM lanes), which share the token columns.
+    const int sub = (warp - 2) >> 2, quarter = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     griddep_wait();
-    int iter = 0;
-    bool gave_up = false;
-    for (int t = cluster; t < tiles && !gave_up; t += clusters, ++iter) {
-      int tn, tt;
+    int iter = 0, buf_at = 0;
+    uint32_t buf_round = 0;
+    bool ok = true;
+    // This thread's channel scales, a tile ahead.
+    float ws_next[Share<T>::kScales];
+    int tn, tt;
+    auto request = [&](int t) {
       tile_of(a, t, tn, tt);
-      const int buf = iter & 1;
-      const int channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
-      const bool live = channel < a.n;
-      const float w_scale = live ? a.w_scale[channel] : 0.f;
-      float* sc = scales + buf * kMaxTok;
-      for (int c = row; c < a.tok; c += kEpiThreads) sc[c] = token0 + c < a.m ? a.x_scale[token0 + c] : 0.f;
-      // One thread waits and the verdict is shared, so that all leave together.  Slot `buf` of verdict
-      // and scales is rewritten two tiles on, after everyone has passed the barrier between.
-      if (row == 0) verdict[buf] = waiter.wait(bar(kBarAccFull + buf), (uint32_t)(iter >> 1) & 1) ? 1 : 0;
-      named_sync(1, kEpiThreads);
-      gave_up = !verdict[buf];
-      if (gave_up || a.splits > 1) break;
-      tc_fence_after();
-      T* y = static_cast<T*>(a.y) + channel;
-      const uint32_t acc = lanes + (uint32_t)(buf * a.acc_cols);
-      for (int c = 0; c < a.tok; c += 16) {
-        uint32_t r[16];
-        tmem_ld16(acc + (uint32_t)c, r);
-        tc_wait_ld();
-        write_columns<T, 16>(a, r, sc, c, token0, y, w_scale, live);
+#pragma unroll
+      for (int j = 0; j < Share<T>::kScales; ++j) {
+        const int ch = (tn * kGroup + half) * kRows + quarter * 32 + Share<T>::channel(j, lane);
+        ws_next[j] = ch < a.n ? a.w_scale[ch] : 0.f;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kGroup == 2)
-          mbar_arrive_cluster(map_to_rank(bar(kBarAccEmpty + buf), (uint32_t)(rank - half)));
-        else
-          mbar_arrive(bar(kBarAccEmpty + buf));
+    };
+    request(cluster);
+    for (int t = cluster; t < tiles && ok; t += clusters, ++iter) {
+      const int buf = iter & 1;
+      const int tn_now = tn, token0 = tt * a.tok;
+      float ws[Share<T>::kScales];
+#pragma unroll
+      for (int j = 0; j < Share<T>::kScales; ++j) ws[j] = ws_next[j];
+      if (t + clusters < tiles) request(t + clusters);
+      ok = waiter.wait_warp(bar(kBarAccFull + buf), (uint32_t)(iter >> 1) & 1);
+      if (!ok || a.splits > 1) break;
+      tc_fence_after();
+      const uint32_t acc = lanes + (uint32_t)(buf * a.acc_cols);
+      auto release = [&]() {  // the accumulator has been read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kGroup == 2)
+            mbar_arrive_cluster(map_to_rank(bar(kBarAccEmpty + buf), (uint32_t)(rank - half)));
+          else
+            mbar_arrive(bar(kBarAccEmpty + buf));
+        }
+      };
+      constexpr int kTok = kBoxTok<T>;
+      for (int c = 0; c < a.tok; c += 2 * kTok) {
+        const int at = c + sub * (kTok / 2);
+        const bool second = c + kTok < a.tok;
+        Share<T> part[2];
+        part[0].load(a, acc + (uint32_t)at, token0 + at, lane);
+        if (second) part[1].load(a, acc + (uint32_t)(at + kTok), token0 + at + kTok, lane);
+        tc_wait_ld();
+        part[0].loaded();
+        part[1].loaded();
+        if (c + 2 * kTok >= a.tok) {  // the accumulator has been read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (kGroup == 2)
+              mbar_arrive_cluster(map_to_rank(bar(kBarAccEmpty + buf), (uint32_t)(rank - half)));
+            else
+              mbar_arrive(bar(kBarAccEmpty + buf));
+          }
+        }
+        if (buf_round > 0) ok = waiter.wait_warp(bar(kBarChunkEmpty + buf_at), (buf_round - 1) & 1);
+        if (!ok) break;
+        const uint32_t stage = staging + (uint32_t)buf_at * kChunkBytes;
+        part[0].put(stage, ws, quarter, sub, lane);
+        if (second) part[1].put(stage + kChunkBytes / 2, ws, quarter, sub, lane);
+        if (a.tma_store) fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kBarChunkFull + buf_at));
+        if (!a.tma_store) {
+          ok = waiter.wait_warp(bar(kBarChunkFull + buf_at), buf_round & 1);
+          if (!ok) break;
+          const int tokens = min(min(2 * kTok, a.tok - c), a.m - token0 - c);
+          const uint8_t* rows = smem_raw + (stage - raw);
+          const int ch = (tn_now * kGroup + half) * kRows;
+          for (int i = warp - 2; i < tokens; i += kEpiWarps)
+            copy_row<T>(rows, i, static_cast<T*>(a.y) + (int64_t)(token0 + c + i) * a.y_stride + ch, a.n - ch, lane);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kBarChunkEmpty + buf_at));
+        }
+        if (++buf_at == kChunkBufs) buf_at = 0, ++buf_round;
       }
     }
-    if (a.splits > 1 && gave_up && row == 0) {
+    if (a.splits > 1 && !ok && lane == 0) {
       for (int r = 0; r < cluster_size; ++r) st_cluster_u1(map_to_rank(tail + kOffPoison, (uint32_t)r) + 4u * split, 1u);
     }
+    __syncwarp();
+  } else if (a.tma_store) {
+    // The store warp: a staged chunk to y by TMA, and its buffer back once it has been read.
+    constexpr int kTok = kBoxTok<T>;
+    const uint32_t elected = elect_one();
+    griddep_wait();
+    int at = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = cluster; t < tiles && ok; t += clusters) {
+      int tn, tt;
+      tile_of(a, t, tn, tt);
+      const int channel0 = (tn * kGroup + half) * kRows, token0 = tt * a.tok;
+      for (int c = 0; c < a.tok; c += 2 * kTok) {
+        ok = waiter.wait_warp(bar(kBarChunkFull + at), phase);
+        if (!ok) break;
+        const uint32_t stage = staging + (uint32_t)at * kChunkBytes;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int token = c + i * kTok;
+          if (token >= a.tok || token0 + token >= a.m) break;
+#pragma unroll
+          for (int b = 0; b < kRows / kBoxChannels<T>; ++b) {
+            const int ch = channel0 + b * kBoxChannels<T>;
+            if (ch < a.n)
+              tma_store_2d(&tm_y, stage + i * (kChunkBytes / 2) + b * kTok * 128, ch, token0 + token, elected);
+          }
+        }
+        if (elected) {
+          bulk_commit_group();
+          bulk_wait_group_read<0>();
+          mbar_arrive(bar(kBarChunkEmpty + at));
+        }
+        __syncwarp();
+        if (++at == kChunkBufs) at = 0, phase ^= 1;
+      }
+    }
+    if (elected) bulk_wait_group0();
     __syncwarp();
   }
 
@@ -328,16 +539,18 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     // One tile per cluster.  Every CTA's MMAs have read their ring, which now takes the parts of the
     // columns that this CTA adds up: groups of 4 token columns, [part][group][channel] x 16 bytes.
     cluster_sync();
-    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const bool epilogue = warp >= 2 && warp < kStoreWarp;
+    const int sub = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
     const int groups = a.tok / 4, per = (groups + a.splits - 1) / a.splits;
     const bool mine_ok = *abort_flag == 0;
-    if (warp >= 2 && mine_ok) {
+    if (epilogue && mine_ok) {
       tc_fence_after();
-      for (int c = 0; c < a.tok; c += 16) {
+      for (int c = sub * 16; c < a.tok; c += 32) {
         uint32_t r[16];
         tmem_ld16(acc + (uint32_t)c, r);
         tc_wait_ld();
+        loaded(r);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int g = c / 4 + j, owner = g / per;
@@ -353,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     cluster_sync();
     bool ok = mine_ok;
     for (int i = 0; i < a.splits; ++i) ok = ok && poison[i] == 0;
-    if (warp >= 2 && ok) {
+    if (epilogue && ok) {
       int tn, tt;
       tile_of(a, cluster, tn, tt);
       const int channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
@@ -361,15 +574,16 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
       const float w_scale = live ? a.w_scale[channel] : 0.f;
       T* y = static_cast<T*>(a.y) + channel;
       const uint8_t* parts = smem_raw + (base - raw) + (size_t)row * 16;
-      for (int g = split * per; g < groups && g < (split + 1) * per; ++g) {
+      for (int g = split * per + sub; g < groups && g < (split + 1) * per; g += 2) {
         uint32_t r[4];
         tmem_ld4(acc + (uint32_t)(4 * g), r);
         tc_wait_ld();
+        loaded(r);
         for (int p = 0; p < a.splits - 1; ++p) {
           const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + g - split * per) * kRows * 16);
           r[0] += v.x, r[1] += v.y, r[2] += v.z, r[3] += v.w;
         }
-        write_columns<T, 4>(a, r, scales, 4 * g, token0, y, w_scale, live);
+        write_columns<T, 4>(a, r, token0 + 4 * g, y, w_scale, live);
       }
     }
     __syncwarp();
@@ -489,7 +703,7 @@ Plan make_plan(int m, int n, int k, int sms) {
   const int n_tiles = (n + kRows * p.group - 1) / (kRows * p.group), t_tiles = (m + p.tok - 1) / p.tok;
   while (p.splits < kMaxSplits / p.group && p.splits * 2 <= k_steps && p.group * n_tiles * t_tiles * p.splits * 2 <= 2 * sms) p.splits *= 2;
   const int stage = kWBytes + p.tok / p.group * kBoxK;
-  const int budget = p.group * n_tiles * t_tiles * p.splits > sms && p.splits > 1 ? 96 * 1024 : 200 * 1024;
+  const int budget = p.group * n_tiles * t_tiles * p.splits > sms && p.splits > 1 ? 96 * 1024 : 192 * 1024;
   p.stages = budget / stage;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   return p;
@@ -509,8 +723,26 @@ int encode(CUtensorMap* map, const void* base, int k, int rows, int64_t stride, 
   return r == CUDA_SUCCESS ? 0 : TMLA_ERR_MISALIGNED;
 }
 
+// The output as a map of its staged boxes.
+template <typename T>
+int encode_y(CUtensorMap* map, const TmlaLinearInt8Params& p) {
+  auto fn = sm100::encode_fn();
+  if (!fn) return TMLA_ERR_CUDA;
+  const CUtensorMapDataType dt = p.dtype == TMLA_DTYPE_FP32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : p.dtype == TMLA_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  cuuint64_t dims[2] = {(cuuint64_t)p.n, (cuuint64_t)p.m};
+  cuuint64_t strides[1] = {(cuuint64_t)p.y_stride * sizeof(T)};
+  cuuint32_t box[2] = {kBoxChannels<T>, kBoxTok<T>};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, dt, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  sizeof(T) == 2 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : TMLA_ERR_MISALIGNED;
+}
+
 template <typename T, int kGroup>
-cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const Args& a, int clusters, size_t smem, bool pdl,
+cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& ty, const Args& a, int clusters, size_t smem, bool pdl,
                       cudaStream_t stream) {
   cudaError_t e =
       cudaFuncSetAttribute(int8_kernel<T, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
@@ -529,7 +761,7 @@ cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const Args& 
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, int8_kernel<T, kGroup>, tw, tx, a);
+  return cudaLaunchKernelEx(&cfg, int8_kernel<T, kGroup>, tw, tx, ty, a);
 }
 
 template <typename T>
@@ -566,10 +798,15 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   if (a.stages < 1 || pl.splits > a.k_steps || pl.splits * pl.group > kMaxSplits || pl.tok > kMaxTok ||
       pl.tok % (16 * pl.group) || (long long)(pl.splits - 1) * per * kRows * 16 > (long long)a.stages * a.stage_bytes)
     return cudaErrorInvalidValue;
-  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + kTailBytes;
+  // TMA stores need rows of y on 16-byte boundaries, and write whole boxes of tokens: past a tile's end only
+  // where that is past y's end too.
+  CUtensorMap ty = tx;
+  a.tma_store = pl.splits == 1 && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
+                p.y_stride * (int64_t)sizeof(T) % 16 == 0 && encode_y<T>(&ty, p) == 0;
+  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + (a.splits == 1 ? kStagingBytes : 0) + kTailBytes;
   const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
-  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, a, clusters, smem, pdl, stream)
-                       : launch_tc<T, 2>(tw, tx, a, clusters, smem, pdl, stream);
+  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, pdl, stream)
+                       : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, pdl, stream);
 }
 
 int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {

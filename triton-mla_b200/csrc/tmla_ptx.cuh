@@ -136,23 +136,32 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
       "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy)
       : "memory");
 }
-// A 2-D tile; its bytes are counted on `bar`.
+// A 2-D tile into this CTA's shared memory, its bytes counted on `bar`.  A converged warp executes it, the
+// thread with `elected` issues it.  kGroup = 2: `bar` (a shared::cluster address) may be the barrier
+// of the pair's other CTA.
+template <int kGroup>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1,
-                                            uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
-      "l"(tmap), "r"(c0), "r"(c1), "r"(bar), "l"(policy)
-      : "memory");
+                                            uint64_t policy, uint32_t elected) {
+  if constexpr (kGroup == 1)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3}], [%4], %5;\n\t}" ::"r"(dst),
+        "l"(tmap), "r"(c0), "r"(c1), "r"(bar), "l"(policy), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint"
+        " [%0], [%1, {%2, %3}], [%4], %5;\n\t}" ::"r"(dst),
+        "l"(tmap), "r"(c0), "r"(c1), "r"(bar), "l"(policy), "r"(elected)
+        : "memory");
 }
-// The same for a CTA pair: the tile goes to this CTA's shared memory, `bar` (a shared::cluster
-// address) may be the pair's other CTA's barrier.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar, int c0, int c1,
-                                                 uint64_t policy) {
+__device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes, uint32_t elected) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint"
-      " [%0], [%1, {%2, %3}], [%4], %5;" ::"r"(dst),
-      "l"(tmap), "r"(c0), "r"(c1), "r"(bar), "l"(policy)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(elected)
       : "memory");
 }
 // Tensor-tile stores from this CTA's shared memory (bulk-group completion).
@@ -165,6 +174,19 @@ __device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int
   asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(tmap),
                "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
+}
+// A 2-D tile from this CTA's shared memory, issued by the thread with `elected` of a converged warp.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int c0, int c1, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n\t}" ::"l"(tmap),
+      "r"(src), "r"(c0), "r"(c1), "r"(elected)
+      : "memory");
+}
+// Wait until all but the last kPending committed bulk stores of this thread have read their shared memory.
+template <int kPending>
+__device__ __forceinline__ void bulk_wait_group_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kPending) : "memory");
 }
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Wait until every committed bulk store of this thread has completed (its writes are done).
@@ -286,40 +308,63 @@ __device__ __forceinline__ void tmem_dealloc_g(uint32_t taddr, uint32_t cols) {
   else
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
 }
-// D(tmem, s32) (+)= A(smem desc, s8) * B(smem desc, s8), K = 32.
-template <int kGroup>
-__device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                       uint32_t accumulate) {
-  if constexpr (kGroup == 1)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// One thread of a converged warp (always the same one).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e;
 }
-// Arrive, when all prior tcgen05 ops of this thread complete, on the mbarrier at this shared-memory
+// D(tmem, s32) (+)= A(smem desc, s8) * B(smem desc, s8), K = 4 x 32: one 128-byte swizzled row of each
+// operand.  A converged warp executes it and the thread with `elected` issues it: the operands
+// are then warp-uniform, which is what the instruction wants (issued from a one-lane branch instead,
+// every operand is moved to a uniform register first, about 66 cycles per MMA).
+template <int kGroup>
+__device__ __forceinline__ void mma_i8_k128(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate, uint32_t elected) {
+#define TMLA_MMA_I8_K128(G)                                                  \
+  asm volatile(                                                              \
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"                         \
+      "setp.ne.b32 p, %4, 0;\n\t"                                            \
+      "setp.ne.b32 q, %5, 0;\n\t"                                            \
+      "@q tcgen05.mma.cta_group::" G ".kind::i8 [%0], %1, %2, %3, p;\n\t"    \
+      "add.s64 a, %1, 2;\n\tadd.s64 b, %2, 2;\n\t"                           \
+      "@q tcgen05.mma.cta_group::" G ".kind::i8 [%0], a, b, %3, 1;\n\t"      \
+      "add.s64 a, %1, 4;\n\tadd.s64 b, %2, 4;\n\t"                           \
+      "@q tcgen05.mma.cta_group::" G ".kind::i8 [%0], a, b, %3, 1;\n\t"      \
+      "add.s64 a, %1, 6;\n\tadd.s64 b, %2, 6;\n\t"                           \
+      "@q tcgen05.mma.cta_group::" G ".kind::i8 [%0], a, b, %3, 1;\n\t}" ::  \
+          "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) \
+      : "memory")
+  if constexpr (kGroup == 1)
+    TMLA_MMA_I8_K128("1");
+  else
+    TMLA_MMA_I8_K128("2");
+#undef TMLA_MMA_I8_K128
+}
+// Arrive, when all prior tcgen05 ops of the elected thread complete, on the mbarrier at this shared-memory
 // offset: this CTA's (kGroup = 1), or those of the cluster's CTAs in `mask` (kGroup = 2).
 template <int kGroup>
-__device__ __forceinline__ void mma_commit_g(uint32_t bar, uint16_t mask) {
+__device__ __forceinline__ void mma_commit_g(uint32_t bar, uint16_t mask, uint32_t elected) {
   if constexpr (kGroup == 1)
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
   else
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            bar),
-        "h"(mask)
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::
+            "r"(bar),
+        "h"(mask), "r"(elected)
         : "memory");
 }
-// 32 lanes x 4 consecutive columns, and x 16: thread i of the warp gets lane (base lane + i).
+// 32 lanes x 4, 8 or 16 consecutive columns: thread i of the warp gets lane (base lane + i).
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_ld4(uint32_t taddr, uint32_t (&r)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -332,6 +377,20 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+// 16 lanes x 16 columns (2 repetitions of 16 lanes x 256 bits), laid out as tmem_ld16x256_x8.
+__device__ __forceinline__ void tmem_ld16x256_x2(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
+// Four 8 x 8 matrices of 16-bit values, transposed: thread t holds of each matrix the values (row t / 4,
+// columns 2 (t % 4) + {0, 1}); column c goes to the 16 bytes at the address that thread 8 j + c gives
+// for matrix j.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 // Stores into another CTA's shared memory (an address from map_to_rank).
 __device__ __forceinline__ void st_cluster_u4(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
