@@ -40,6 +40,7 @@ struct Args {
   int64_t m;
   int k;
   float eps;
+  bool early_w;  // the preceding kernel does not write w
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -196,15 +197,19 @@ __global__ void __launch_bounds__(kVecs >= 4 ? 512 : kMaxThreads, kVecs == 4 ? 2
   const uint4 zero = make_uint4(0, 0, 0, 0);
   uint4 w[kNorm ? kVecs : 1];
   float w_last = 0.f;
-  if constexpr (kNorm) {
+  auto load_weight = [&]() {
     const T* wp = static_cast<const T*>(a.w);
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
       w[i] = i * threads + t < vecs ? reinterpret_cast<const uint4*>(wp)[i * threads + t] : zero;
     if (last >= 0) w_last = to_float(wp[last]);
-  }
+  };
+  if constexpr (kNorm)
+    if (a.early_w) load_weight();
   ptx::griddep_wait();
   ptx::griddep_launch_dependents();
+  if constexpr (kNorm)
+    if (!a.early_w) load_weight();
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   uint4 h[kVecs];
   float h_last = 0.f;
@@ -334,8 +339,10 @@ __global__ void __launch_bounds__(kMaxThreads) loop_kernel(const Args a) {
 
 // ---------------------------------------------------------------------------- host side
 
+// A programmatic launch: the kernel may be scheduled while the one before it in the stream finishes, and
+// waits for it (griddepcontrol.wait) before it touches memory.
 template <typename K>
-cudaError_t launch(K kernel, dim3 grid, dim3 block, const Args& a, bool pdl, cudaStream_t stream) {
+cudaError_t launch(K kernel, dim3 grid, dim3 block, const Args& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -344,17 +351,17 @@ cudaError_t launch(K kernel, dim3 grid, dim3 block, const Args& a, bool pdl, cud
   cfg.blockDim = block;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <typename T, bool kNorm>
-cudaError_t run(const Args& a, bool aligned, bool pdl, cudaStream_t stream) {
+cudaError_t run(const Args& a, bool aligned, cudaStream_t stream) {
   const int vecs = a.k / kPer<T> > 0 ? a.k / kPer<T> : 1;
   if (!aligned || vecs > 8 * 512) {
     const int threads = a.k < kMaxThreads ? (a.k + 31) / 32 * 32 : kMaxThreads;
-    return aligned ? launch(loop_kernel<T, kNorm, true>, dim3((unsigned)a.m), dim3(threads), a, pdl, stream)
-                   : launch(loop_kernel<T, kNorm, false>, dim3((unsigned)a.m), dim3(threads), a, pdl, stream);
+    return aligned ? launch(loop_kernel<T, kNorm, true>, dim3((unsigned)a.m), dim3(threads), a, stream)
+                   : launch(loop_kernel<T, kNorm, false>, dim3((unsigned)a.m), dim3(threads), a, stream);
   }
   // Vectors per thread (bf16 on B200, us per call): 4 keep more loads in flight than 1 or 2 (norm with
   // residual of 8192 x 7168: 72.7 against 98.3 and 96.1; 4096 x 16384: 84.7 against 115), and 8
@@ -367,10 +374,10 @@ cudaError_t run(const Args& a, bool aligned, bool pdl, cudaStream_t stream) {
   const int rows = threads >= 128 ? 1 : 128 / threads;
   const dim3 grid((unsigned)((a.m + rows - 1) / rows)), block(threads, rows);
   switch (per) {
-    case 1: return launch(rows_kernel<T, 1, kNorm>, grid, block, a, pdl, stream);
-    case 2: return launch(rows_kernel<T, 2, kNorm>, grid, block, a, pdl, stream);
-    case 4: return launch(rows_kernel<T, 4, kNorm>, grid, block, a, pdl, stream);
-    default: return launch(rows_kernel<T, 8, kNorm>, grid, block, a, pdl, stream);
+    case 1: return launch(rows_kernel<T, 1, kNorm>, grid, block, a, stream);
+    case 2: return launch(rows_kernel<T, 2, kNorm>, grid, block, a, stream);
+    case 4: return launch(rows_kernel<T, 4, kNorm>, grid, block, a, stream);
+    default: return launch(rows_kernel<T, 8, kNorm>, grid, block, a, stream);
   }
 }
 
@@ -409,18 +416,18 @@ int start(const TmlaInt8RowsParams& p, bool norm, void* stream) {
               (!norm || (uintptr_t)p.weight % 16 == 0) &&
               (!res || (rows_aligned(p.residual, p.residual_stride, size, 16) &&
                         rows_aligned(p.h, p.h_stride, size, 16)));
-  const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
+  a.early_w = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (p.dtype) {
     case TMLA_DTYPE_BF16:
-      e = norm ? run<__nv_bfloat16, true>(a, aligned, pdl, s) : run<__nv_bfloat16, false>(a, aligned, pdl, s);
+      e = norm ? run<__nv_bfloat16, true>(a, aligned, s) : run<__nv_bfloat16, false>(a, aligned, s);
       break;
     case TMLA_DTYPE_FP16:
-      e = norm ? run<__half, true>(a, aligned, pdl, s) : run<__half, false>(a, aligned, pdl, s);
+      e = norm ? run<__half, true>(a, aligned, s) : run<__half, false>(a, aligned, s);
       break;
     default:
-      e = norm ? run<float, true>(a, aligned, pdl, s) : run<float, false>(a, aligned, pdl, s);
+      e = norm ? run<float, true>(a, aligned, s) : run<float, false>(a, aligned, s);
       break;
   }
   if (e == cudaSuccess) e = cudaGetLastError();

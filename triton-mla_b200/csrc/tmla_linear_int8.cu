@@ -23,6 +23,7 @@
 // frees TMEM and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+#include <math.h>
 
 #include "tmla_common.cuh"
 #include "tmla_ptx.cuh"
@@ -58,13 +59,11 @@ constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 // After the ring and the staged chunks: barriers full / empty per stage, accumulator full / empty (two),
-// "MMAs done", chunk full / empty; the TMEM address, the abort flag, the gave-up flags of the
-// cluster's parts.
+// "MMAs done", chunk full / empty, the parts of a split tile; the TMEM address, the abort flag.
 constexpr int kBarFull = 0, kBarEmpty = kMaxStages, kBarAccFull = 2 * kMaxStages, kBarAccEmpty = kBarAccFull + 2,
               kBarMmaDone = kBarAccEmpty + 2, kBarChunkFull = kBarMmaDone + 1, kBarChunkEmpty = kBarChunkFull + kChunkBufs,
-              kNumBars = kBarChunkEmpty + kChunkBufs;
-constexpr uint32_t kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4, kOffPoison = kOffAbort + 4,
-                   kTailBytes = kOffPoison + 4 * kMaxSplits;
+              kBarParts = kBarChunkEmpty + kChunkBufs, kNumBars = kBarParts + 1;
+constexpr uint32_t kOffTmem = 8 * kNumBars, kOffAbort = kOffTmem + 4, kTailBytes = kOffAbort + 4;
 
 struct Args {
   int m, n;
@@ -72,6 +71,7 @@ struct Args {
   int n_tiles, t_tiles;     // tiles of channels and of tokens
   int k_steps;
   int stages, stage_bytes, x_bytes;  // x_bytes: this CTA's token rows of a stage
+  int staging_bytes;        // staged chunks of y, or the parts sent by the cluster's other CTAs
   int acc_cols, tmem_cols;  // TMEM columns of an accumulator, and allocated
   int tma_store;            // y's rows start on 16-byte boundaries: TMA stores (else copied by the epilogue)
   int band;                 // token tiles walked together (see tile_of)
@@ -81,6 +81,7 @@ struct Args {
   int64_t y_stride;
   int* status;
   unsigned long long wait_ns;
+  int early_w;              // the preceding kernel does not write w
   int stall;                // test only: the first CTA never loads its first stage
 };
 
@@ -273,11 +274,10 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t staging = base + (uint32_t)(a.stages * a.stage_bytes);
-  const uint32_t tail = staging + (a.splits == 1 ? kStagingBytes : 0);
+  const uint32_t tail = staging + (uint32_t)a.staging_bytes;
   uint8_t* tail_ptr = smem_raw + (tail - raw);
   auto bar = [&](int i) { return tail + 8u * (uint32_t)i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tail_ptr + kOffAbort);
-  volatile int* poison = reinterpret_cast<volatile int*>(tail_ptr + kOffPoison);
 
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int cluster_size = kGroup * a.splits;
@@ -286,83 +286,90 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   const bool leader = half == 0;
   const int cluster = (int)blockIdx.x / cluster_size, clusters = (int)gridDim.x / cluster_size;
   const int tiles = a.n_tiles * a.t_tiles;
+  // The token columns of a split tile in groups of 4: `per` for each part, of which this part adds up parts_here.
+  const int per = (a.tok / 4 + a.splits - 1) / a.splits;
+  const int parts_here = a.splits > 1 ? max(0, min(per, a.tok / 4 - split * per)) : 0;
   const int ks0 = (int)((long long)split * a.k_steps / a.splits);
   const int ks1 = (int)((long long)(split + 1) * a.k_steps / a.splits);
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; ++s) {
-      mbar_init(bar(kBarFull + s), 1);
-      mbar_init(bar(kBarEmpty + s), 1);
+  // Warp 0's part before the roles start: the barriers, and the loads of the first round of the ring.
+  const uint32_t elected = elect_one();
+  const bool stalled = a.stall && blockIdx.x == 0;
+  // A weight row is used by one token tile only, or again by the next ones.
+  const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
+  const uint64_t pol_x = policy_evict_last();
+  const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
+  auto load_w = [&](int s, int ks, int row) {
+    if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), (uint32_t)(kGroup * (kWBytes + a.x_bytes)), elected);
+    tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes), &tm_w, pair_bar + 8u * (uint32_t)(kBarFull + s),
+                        ks * kBoxK, row, pol_w, elected);
+  };
+  auto load_x = [&](int s, int ks, int row) {
+    tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes + kWBytes), &tm_x,
+                        pair_bar + 8u * (uint32_t)(kBarFull + s), ks * kBoxK, row, pol_x, elected);
+  };
+  const int pre = ks1 - ks0 < a.stages ? ks1 - ks0 : a.stages;
+  auto first_round = [&]() {
+    int tn, tt;
+    tile_of(a, cluster, tn, tt);
+    const int w_row = (tn * kGroup + half) * kRows, x_row = tt * a.tok + half * (a.tok / kGroup);
+    // With the caller's word that the kernel before does not write w, the weight boxes of two stages are
+    // requested before it has completed; more of them would delay its own loads.
+    const int early = !a.early_w ? 0 : pre < 2 ? pre : 2;
+    for (int s = 0; s < early; ++s)
+      if (!stalled || s > 0) load_w(s, ks0 + s, w_row);
+    griddep_wait();
+    for (int s = 0; s < pre; ++s) {
+      if (s >= early && (!stalled || s > 0)) load_w(s, ks0 + s, w_row);
+      if (!stalled || s > 0) load_x(s, ks0 + s, x_row);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(kBarAccFull + b), 1);
-      mbar_init(bar(kBarAccEmpty + b), kGroup * kEpiWarps);
+  };
+  if (warp == 0) {
+    for (int i = lane; i < kNumBars; i += 32) {
+      const int count = i >= kBarAccEmpty && i < kBarMmaDone       ? kGroup * kEpiWarps
+                        : i >= kBarChunkFull && i < kBarChunkEmpty ? kEpiWarps
+                        : i >= kBarChunkEmpty && i < kBarParts     ? (a.tma_store ? 1 : kEpiWarps)
+                                                                   : 1;
+      mbar_init(bar(i), (uint32_t)count);
     }
-    for (int b = 0; b < kChunkBufs; ++b) {
-      mbar_init(bar(kBarChunkFull + b), kEpiWarps);
-      mbar_init(bar(kBarChunkEmpty + b), a.tma_store ? 1 : kEpiWarps);
-    }
-    mbar_init(bar(kBarMmaDone), 1);
-    *abort_flag = 0;
-    for (int i = 0; i < kMaxSplits; ++i) poison[i] = 0;
+    if (lane == 0) *abort_flag = 0;
     fence_mbar_init();
-    prefetch_tmap(&tm_w);
-    prefetch_tmap(&tm_x);
-  }
-  if (warp == 1) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (parts_here > 0)
+      mbar_arrive_expect_tx(bar(kBarParts), (uint32_t)((a.splits - 1) * parts_here * kRows * 16), elected);
+    if (kGroup == 1) first_round();  // a single CTA's loads concern nobody else
+  } else if (warp == 1) {
     tmem_alloc_g<kGroup>(tail + kOffTmem, (uint32_t)a.tmem_cols);
     tmem_relinquish_g<kGroup>();
   }
   tc_fence_before();
-  if (cluster_size > 1)
-    cluster_sync();
-  else
-    __syncthreads();
+  __syncthreads();
+  // The cluster's CTAs have set up their barriers when this completes: a pair needs that at once, the parts
+  // of a split tile before they are sent.
+  if (cluster_size > 1) cluster_arrive();
+  if (kGroup == 2) cluster_wait();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tail_ptr + kOffTmem);
   const Waiter waiter{abort_flag, a.status, a.wait_ns};
 
   if (warp == 0) {
-    // The whole warp runs this (its operands stay warp-uniform); one thread issues.
-    const uint32_t elected = elect_one();
-    const bool stalled = a.stall && blockIdx.x == 0;
-    // A weight row is used by one token tile only, or again by the next ones.
-    const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
-    const uint64_t pol_x = policy_evict_last();
-    const uint32_t tx = (uint32_t)(kGroup * (kWBytes + a.x_bytes));
-    const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
-    auto load_w = [&](int s, int ks, int row) {
-      tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes), &tm_w, pair_bar + 8u * (uint32_t)(kBarFull + s),
-                          ks * kBoxK, row, pol_w, elected);
-    };
-    // The weight boxes of the first stages do not depend on the kernel before (a programmatic
-    // launch): they are requested before it has completed.
-    int tn, tt;
-    tile_of(a, cluster, tn, tt);
-    const int pre = ks1 - ks0 < a.stages ? ks1 - ks0 : a.stages, early = pre < 2 ? pre : 2;
-    for (int j = 0; j < early; ++j) {
-      if (stalled && j == 0) continue;
-      if (leader) mbar_arrive_expect_tx(bar(kBarFull + j), tx, elected);
-      load_w(j, ks0 + j, (tn * kGroup + half) * kRows);
-    }
-    griddep_wait();
+    // Past this the next kernel may be scheduled; this CTA holds its TMEM already, so it cannot be kept out.
     griddep_launch_dependents();
-    int s = 0;           // ring position, and how often the ring has wrapped
-    uint32_t round = 0;
+    // The whole warp runs this (its operands stay warp-uniform); one thread issues.
+    if (kGroup == 2) first_round();
+    int s = pre == a.stages ? 0 : pre;               // ring position, and how often the ring has wrapped
+    uint32_t round = pre == a.stages ? 1 : 0;
     bool ok = true;
     for (int t = cluster; t < tiles && ok; t += clusters) {
+      int tn, tt;
       tile_of(a, t, tn, tt);
       const int w_row = (tn * kGroup + half) * kRows, x_row = tt * a.tok + half * (a.tok / kGroup);
-      for (int ks = ks0; ks < ks1; ++ks) {
+      for (int ks = t == cluster ? ks0 + pre : ks0; ks < ks1; ++ks) {
         if (round > 0) ok = waiter.wait_warp(bar(kBarEmpty + s), (round - 1) & 1);
         if (!ok) break;
-        if (round > 0 || s >= early) {
-          if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), tx, elected);
-          load_w(s, ks, w_row);
-        }
-        if (!stalled || round > 0 || s > 0)
-          tma_load_2d<kGroup>(base + (uint32_t)(s * a.stage_bytes) + kWBytes, &tm_x,
-                              pair_bar + 8u * (uint32_t)(kBarFull + s), ks * kBoxK, x_row, pol_x, elected);
+        load_w(s, ks, w_row);
+        load_x(s, ks, x_row);
         if (++s == a.stages) s = 0, ++round;
       }
     }
@@ -376,7 +383,6 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   } else if (warp == 1) {
     // The whole warp runs this (its operands stay warp-uniform); one thread issues.
     if (leader) {
-      const uint32_t elected = elect_one();
       const uint32_t idesc = idesc_i8(kRows * kGroup, (uint32_t)a.tok);
       const uint16_t mask = (uint16_t)(3u << (rank - half));
       int iter = 0, s = 0;
@@ -393,7 +399,8 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
           if (!ok) break;
           tc_fence_after();
           const uint32_t st = base + (uint32_t)(s * a.stage_bytes);
-          mma_i8_k128<kGroup>(d, smem_desc(st, 16, 1024, kSwizzle128B), smem_desc(st + kWBytes, 16, 1024, kSwizzle128B),
+          mma_i8_k128<kGroup>(d, smem_desc(st, 16, 1024, kSwizzle128B),
+                              smem_desc(st + kWBytes, 16, 1024, kSwizzle128B),
                               idesc, ks > ks0 ? 1u : 0u, elected);
           issued = true;
           mma_commit_g<kGroup>(bar(kBarEmpty + s), mask, elected);
@@ -482,23 +489,64 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
           if (!ok) break;
           const int tokens = min(min(2 * kTok, a.tok - c), a.m - token0 - c);
           const uint8_t* rows = smem_raw + (stage - raw);
-          const int ch = (tn_now * kGroup + half) * kRows;
+          const int ch = (tn_now * kGroup + half) * kRows, left = a.n - ch;
           for (int i = warp - 2; i < tokens; i += kEpiWarps)
-            copy_row<T>(rows, i, static_cast<T*>(a.y) + (int64_t)(token0 + c + i) * a.y_stride + ch, a.n - ch, lane);
+            copy_row<T>(rows, i, static_cast<T*>(a.y) + (int64_t)(token0 + c + i) * a.y_stride + ch, left, lane);
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(kBarChunkEmpty + buf_at));
         }
         if (++buf_at == kChunkBufs) buf_at = 0, ++buf_round;
       }
     }
-    if (a.splits > 1 && !ok && lane == 0) {
-      for (int r = 0; r < cluster_size; ++r) st_cluster_u1(map_to_rank(tail + kOffPoison, (uint32_t)r) + 4u * split, 1u);
+    if (a.splits > 1) {
+      // One tile per cluster: this part's columns to the CTAs that add them up, in groups of 4 token
+      // columns, [part][group][channel] x 16 bytes, which complete on their barrier.
+      const int row = quarter * 32 + lane, channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
+      const bool live = channel < a.n;
+      const float w_scale = live ? a.w_scale[channel] : 0.f;
+      if (kGroup == 1) cluster_wait();
+      if (ok) {
+        tc_fence_after();
+        for (int c = sub * 16; c < a.tok; c += 32) {
+          uint32_t r[16];
+          tmem_ld16(lanes + (uint32_t)c, r);
+          tc_wait_ld();
+          loaded(r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int g = c / 4 + j, owner = g / per;
+            if (owner == split) continue;
+            const int part = split < owner ? split : split - 1;
+            const uint32_t to = (uint32_t)(owner * kGroup + half);
+            st_async_u4(map_to_rank(staging + (uint32_t)(((part * per + g - owner * per) * kRows + row) * 16), to),
+                        make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]),
+                        map_to_rank(bar(kBarParts), to));
+          }
+        }
+      }
+      __syncwarp();
+      cluster_arrive();  // everything sent; completed at the end, before any CTA exits
+      if (parts_here > 0 && ok && waiter.wait_warp<true>(bar(kBarParts), 0)) {
+        T* y = static_cast<T*>(a.y) + channel;
+        const uint8_t* parts = smem_raw + (staging - raw) + (size_t)row * 16;
+        for (int i = sub; i < parts_here; i += 2) {
+          const int g = split * per + i;
+          uint32_t r[4];
+          tmem_ld4(lanes + (uint32_t)(4 * g), r);
+          tc_wait_ld();
+          loaded(r);
+          for (int p = 0; p < a.splits - 1; ++p) {
+            const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + i) * kRows * 16);
+            r[0] += v.x, r[1] += v.y, r[2] += v.z, r[3] += v.w;
+          }
+          write_columns<T, 4>(a, r, token0 + 4 * g, y, w_scale, live);
+        }
+      }
     }
     __syncwarp();
   } else if (a.tma_store) {
     // The store warp: a staged chunk to y by TMA, and its buffer back once it has been read.
     constexpr int kTok = kBoxTok<T>;
-    const uint32_t elected = elect_one();
     griddep_wait();
     int at = 0;
     uint32_t phase = 0;
@@ -535,65 +583,17 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     __syncwarp();
   }
 
-  if (a.splits > 1) {
-    // One tile per cluster.  Every CTA's MMAs have read their ring, which now takes the parts of the
-    // columns that this CTA adds up: groups of 4 token columns, [part][group][channel] x 16 bytes.
-    cluster_sync();
-    const bool epilogue = warp >= 2 && warp < kStoreWarp;
-    const int sub = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
-    const int groups = a.tok / 4, per = (groups + a.splits - 1) / a.splits;
-    const bool mine_ok = *abort_flag == 0;
-    if (epilogue && mine_ok) {
-      tc_fence_after();
-      for (int c = sub * 16; c < a.tok; c += 32) {
-        uint32_t r[16];
-        tmem_ld16(acc + (uint32_t)c, r);
-        tc_wait_ld();
-        loaded(r);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int g = c / 4 + j, owner = g / per;
-          if (owner == split) continue;
-          const int part = split < owner ? split : split - 1;
-          const uint32_t at = base + (uint32_t)(((part * per + g - owner * per) * kRows + row) * 16);
-          st_cluster_u4(map_to_rank(at, (uint32_t)(owner * kGroup + half)), r[4 * j], r[4 * j + 1], r[4 * j + 2],
-                        r[4 * j + 3]);
-        }
-      }
+  __syncwarp();
+  if (cluster_size > 1) {
+    // No CTA exits while another may still write to its shared memory or use its half of a pair's operands.
+    if (a.splits == 1 || warp < 2 || warp == kStoreWarp) {
+      if (kGroup == 1) cluster_wait();
+      cluster_arrive();
     }
-    __syncwarp();
-    cluster_sync();
-    bool ok = mine_ok;
-    for (int i = 0; i < a.splits; ++i) ok = ok && poison[i] == 0;
-    if (epilogue && ok) {
-      int tn, tt;
-      tile_of(a, cluster, tn, tt);
-      const int channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
-      const bool live = channel < a.n;
-      const float w_scale = live ? a.w_scale[channel] : 0.f;
-      T* y = static_cast<T*>(a.y) + channel;
-      const uint8_t* parts = smem_raw + (base - raw) + (size_t)row * 16;
-      for (int g = split * per + sub; g < groups && g < (split + 1) * per; g += 2) {
-        uint32_t r[4];
-        tmem_ld4(acc + (uint32_t)(4 * g), r);
-        tc_wait_ld();
-        loaded(r);
-        for (int p = 0; p < a.splits - 1; ++p) {
-          const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + g - split * per) * kRows * 16);
-          r[0] += v.x, r[1] += v.y, r[2] += v.z, r[3] += v.w;
-        }
-        write_columns<T, 4>(a, r, token0 + 4 * g, y, w_scale, live);
-      }
-    }
-    __syncwarp();
+    cluster_wait();
   }
-
   tc_fence_before();
-  if (cluster_size > 1)
-    cluster_sync();
-  else
-    __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_g<kGroup>(tmem, (uint32_t)a.tmem_cols);
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(256) generic_kernel(const GenericArgs a) {
 }
 
 template <typename T>
-cudaError_t launch_generic(const GenericArgs& a, bool pdl, cudaStream_t stream) {
+cudaError_t launch_generic(const GenericArgs& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -678,7 +678,7 @@ cudaError_t launch_generic(const GenericArgs& a, bool pdl, cudaStream_t stream) 
   cfg.blockDim = dim3(256);
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, generic_kernel<T>, a);
 }
 
@@ -687,6 +687,11 @@ struct Plan {
   int group, tok, splits, stages;
 };
 
+// The parts of a split tile's columns that a CTA receives, or the staged chunks of y.
+int staging_bytes(const Plan& p) {
+  return p.splits == 1 ? (int)kStagingBytes : (p.splits - 1) * ((p.tok / 4 + p.splits - 1) / p.splits) * kRows * 16;
+}
+
 int sm_count() {
   int dev = 0, v = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -694,19 +699,52 @@ int sm_count() {
   return v;
 }
 
+// Estimated microseconds of a call as waves of tiles.  A k-step takes the longest of its MMAs, the
+// shared-memory fill of a CTA and a fixed time; a tile its k-steps or, unsplit, the epilogue of the
+// tile before it; the whole at least HBM's time for the operands and y.  The constants are fitted to 1,500
+// calls measured on B200 (1 to 4096 tokens, eight n x k from 512 x 16384 to 20000 x 128, all variants,
+// bf16 out): the variant with the least estimate is on average 1.4% slower than the fastest measured,
+// 11% at worst.
+double estimate(int m, int n, int k, int group, int tok, int splits, int sms) {
+  const double k_steps = (k + kBoxK - 1) / kBoxK, tiles = (double)((n + kRows * group - 1) / (kRows * group)) *
+                                                          ((m + tok - 1) / tok);
+  // Clusters of 1 to 8 CTAs that run at once on 148 SMs with one CTA each (the occupancy calculator's).
+  constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+  const double slots = kClusters[group * splits] * (sms / 148.0);
+  const double step = fmax(fmax(1.08 * tok, 8.06 * (16 + tok / 8.0 / group)), 157.) * 1e-3;
+  const double epilogue = (5.3 * tok + 664.) * 1e-3, steps = ceil(k_steps / splits) * step;
+  const double tiles_us = ceil(tiles / slots) * (splits == 1 ? fmax(steps, epilogue) : steps);
+  const double hbm_us = ((double)n * k + (double)m * k + 1.8 * m * n) / 4.25e6;
+  return (group == 2 ? 0.69 : 0.) + fmax(tiles_us, hbm_us) + 0.11 * fmin(tiles_us, hbm_us) +
+         (splits == 1 ? epilogue : 0.36 + 0.029 * tok);
+}
+
+// The variant with the least estimate.  Examples (us measured, chosen against the next kind):
+//   16 tokens, wo (7168 x 16384): 2 parts 23.9, unsplit 24.5, CTA pairs 24.8;
+//   16 tokens, [wq_a; wkv_a] (2112 x 7168): 6 parts 6.9, unsplit 10.4;
+//   256 tokens, wo: pairs of 128 tokens 32.0, single CTAs 33.9;  4096 tokens, wq_b: pairs of 256 113, single 122;
+//   4096 tokens, 20000 x 128: single CTAs 50, pairs 58.
 Plan make_plan(int m, int n, int k, int sms) {
-  Plan p;
+  constexpr int kTokens[] = {64, 96, 128, 192, 256}, kSplits[] = {1, 2, 3, 4, 6};
+  Plan best{};
+  double least = 0;
   const int k_steps = (k + kBoxK - 1) / kBoxK;
-  p.group = m <= 128 ? 1 : 2;
-  p.tok = p.group == 1 ? (m <= 64 ? (m + 15) / 16 * 16 : (m + 31) / 32 * 32) : 256;
-  p.splits = 1;
-  const int n_tiles = (n + kRows * p.group - 1) / (kRows * p.group), t_tiles = (m + p.tok - 1) / p.tok;
-  while (p.splits < kMaxSplits / p.group && p.splits * 2 <= k_steps && p.group * n_tiles * t_tiles * p.splits * 2 <= 2 * sms) p.splits *= 2;
-  const int stage = kWBytes + p.tok / p.group * kBoxK;
-  const int budget = p.group * n_tiles * t_tiles * p.splits > sms && p.splits > 1 ? 96 * 1024 : 192 * 1024;
-  p.stages = budget / stage;
-  if (p.stages > kMaxStages) p.stages = kMaxStages;
-  return p;
+  for (int group = 1; group <= 2; ++group) {
+    for (int i = 0; i < 5; ++i) {
+      // Up to 64 tokens one tile holds them all, in steps of the MMA's N.
+      const int step = 16 * group, tok = m <= 64 ? (m + step - 1) / step * step : kTokens[i];
+      if (i > 0 && (m <= 64 || kTokens[i - 1] >= m)) break;
+      for (const int splits : kSplits) {
+        if (splits * group > kMaxSplits || splits > k_steps) break;
+        const double t = estimate(m, n, k, group, tok, splits, sms);
+        if (best.group == 0 || t < least) best = Plan{group, tok, splits, 0}, least = t;
+      }
+    }
+  }
+  const int stage = (kRows + best.tok / best.group) * kBoxK;
+  best.stages = ((int)(kSmemMax - 1024 - kTailBytes) - staging_bytes(best)) / stage;
+  if (best.stages > kMaxStages) best.stages = kMaxStages;
+  return best;
 }
 
 // A matrix of int8 rows as a map of boxes of `rows` rows x 128 swizzled bytes; outside it reads zeros.
@@ -742,8 +780,8 @@ int encode_y(CUtensorMap* map, const TmlaLinearInt8Params& p) {
 }
 
 template <typename T, int kGroup>
-cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& ty, const Args& a, int clusters, size_t smem, bool pdl,
-                      cudaStream_t stream) {
+cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& ty, const Args& a, int clusters,
+                      size_t smem, cudaStream_t stream) {
   cudaError_t e =
       cudaFuncSetAttribute(int8_kernel<T, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
   if (e != cudaSuccess) return e;
@@ -760,7 +798,7 @@ cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtens
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 2 : 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, int8_kernel<T, kGroup>, tw, tx, ty, a);
 }
 
@@ -777,7 +815,8 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   a.k_steps = (p.k + kBoxK - 1) / kBoxK;
   a.x_bytes = pl.tok / pl.group * kBoxK;
   a.stages = pl.stages;
-  a.stage_bytes = kWBytes + a.x_bytes;
+  a.stage_bytes = kRows * kBoxK + a.x_bytes;
+  a.staging_bytes = staging_bytes(pl);
   const int tiles = a.n_tiles * a.t_tiles;
   const int resident = sms / pl.group;
   const int clusters = pl.splits > 1 || tiles < resident ? tiles : resident;
@@ -791,22 +830,20 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   a.y_stride = p.y_stride;
   a.status = p.status;
   a.wait_ns = p.wait_ns > 0 ? (unsigned long long)p.wait_ns : kWaitNs;
+  a.early_w = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
   a.stall = (p.flags & TMLA_LINEAR_FLAG_TEST_STALL) ? 1 : 0;
-  // What the kernel takes for granted: a ring, at least one k-step per part, the parts of the columns that a
-  // CTA adds up fit into the ring.
-  const int per = (pl.tok / 4 + pl.splits - 1) / pl.splits;
+  // What the kernel takes for granted.
   if (a.stages < 1 || pl.splits > a.k_steps || pl.splits * pl.group > kMaxSplits || pl.tok > kMaxTok ||
-      pl.tok % (16 * pl.group) || (long long)(pl.splits - 1) * per * kRows * 16 > (long long)a.stages * a.stage_bytes)
+      pl.tok % (16 * pl.group))
     return cudaErrorInvalidValue;
   // TMA stores need rows of y on 16-byte boundaries, and write whole boxes of tokens: past a tile's end only
   // where that is past y's end too.
   CUtensorMap ty = tx;
   a.tma_store = pl.splits == 1 && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
                 p.y_stride * (int64_t)sizeof(T) % 16 == 0 && encode_y<T>(&ty, p) == 0;
-  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + (a.splits == 1 ? kStagingBytes : 0) + kTailBytes;
-  const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
-  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, pdl, stream)
-                       : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, pdl, stream);
+  const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + a.staging_bytes + kTailBytes;
+  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, stream)
+                       : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, stream);
 }
 
 int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
@@ -817,15 +854,14 @@ int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
   if (p.m == 0 || p.n == 0) return TMLA_OK;
   if (!p.x || !p.x_scale || !p.w || !p.w_scale || !p.y) return TMLA_ERR_INVALID_ARG;
   if (p.x_stride < p.k || p.w_stride < p.k || p.y_stride < p.n) return TMLA_ERR_INVALID_ARG;
-  const bool pdl = (p.flags & TMLA_LAYER_FLAG_PDL) != 0;
   cudaError_t e;
   if ((((uintptr_t)p.x | (uintptr_t)p.w) % 16 || p.x_stride % 16 || p.w_stride % 16)) {
     const GenericArgs a{static_cast<const int8_t*>(p.x), p.x_stride, p.x_scale, static_cast<const int8_t*>(p.w),
                         p.w_stride, p.w_scale, p.y, p.y_stride, p.m, p.n, p.k};
     switch (p.dtype) {
-      case TMLA_DTYPE_BF16: e = launch_generic<__nv_bfloat16>(a, pdl, stream); break;
-      case TMLA_DTYPE_FP16: e = launch_generic<__half>(a, pdl, stream); break;
-      default: e = launch_generic<float>(a, pdl, stream); break;
+      case TMLA_DTYPE_BF16: e = launch_generic<__nv_bfloat16>(a, stream); break;
+      case TMLA_DTYPE_FP16: e = launch_generic<__half>(a, stream); break;
+      default: e = launch_generic<float>(a, stream); break;
     }
   } else {
     const int sms = sm_count();
