@@ -114,4 +114,4 @@ def test_int8_operators_have_meta_kernels():
     assert ops.rms_norm_int8(x, w, 1e-6, None, None, False)[2].numel() == 0
     wq = torch.empty(70, 1001, dtype=torch.int8, device="meta")
     y = ops.linear_int8(q, scale, wq, torch.empty(70, device="meta"), torch.float16, False, None)
-    assert y.shape == (5, 70) and y.dtype == torch.float16
+    assert y.shape == (5, 70) and y.dtype == torch.float16 and y.stride() == (72, 1)

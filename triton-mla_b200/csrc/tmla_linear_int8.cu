@@ -42,18 +42,21 @@ constexpr int kWBytes = kRows * kBoxK;     // weight bytes of a stage
 constexpr int kMaxTok = 256;               // tokens per tile (MMA N)
 constexpr int kMaxSplits = 8;              // CTAs of a portable cluster
 constexpr int kMaxStages = 12;
+// Stages whose weights are requested into L2 before the kernel before has ended.  Four, all, none (us on
+// B200): wo 16 tokens 22.5, 22.3, 23.1; rms_norm_int8 and [wq_a; wkv_a] in a row 8.6, 9.3, 9.1.
+constexpr int kPrefetch = 4;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
 constexpr int kStoreWarp = 2 + kEpiWarps;
 constexpr int kThreads = 32 * (kStoreWarp + 1);
-// y leaves in chunks of 128 channels x 2 kBoxTok<T> tokens, staged in shared memory as boxes of 128 bytes
-// of channels x kBoxTok<T> tokens.
+// y leaves in chunks of 128 channels x 2 kBoxTok<T> tokens, staged in shared memory as boxes of
+// kBoxChannels<T> channels (128 bytes of 16-bit values, swizzled; all 128 of fp32) x kBoxTok<T> tokens.
 constexpr uint32_t kChunkBytes = 16384;
 constexpr int kChunkBufs = 2;
 constexpr uint32_t kStagingBytes = kChunkBufs * kChunkBytes;
 template <typename T>
 constexpr int kBoxTok = (int)(kChunkBytes / (2 * kRows * sizeof(T)));  // 32 of 16 bits, 16 of fp32
 template <typename T>
-constexpr int kBoxChannels = (int)(128 / sizeof(T));
+constexpr int kBoxChannels = sizeof(T) == 2 ? 64 : kRows;
 constexpr int kMaxRows = 1 << 30;          // tokens and channels: row numbers past a tile's end stay in int
 constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -172,23 +175,25 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[N]) {
 // A warp's share of a box of tokens: its 32 channels x half of the tokens, from `token` and `acc` on.
 // 16-bit y: 16 tokens.  The 16x256b loads leave the accumulator in the registers as 8 x 8 matrices of
 // channels x tokens, which stmatrix writes transposed into 128-byte swizzled rows of 64 channels.
-// fp32 y: 8 tokens, a thread's channel straight into rows of 32 channels.
+// fp32 y: 8 tokens, a thread's channel straight into rows of 128 channels.
+// `scales` holds the scale of box token i in thread i.
 template <typename T>
 struct Share {
   uint32_t r[16];
-  float s[4];
-  __device__ __forceinline__ void load(const Args& a, uint32_t acc, int token, int lane) {
+  __device__ __forceinline__ void load(uint32_t acc) {
     tmem_ld16x256_x2(acc, *reinterpret_cast<uint32_t(*)[8]>(r));
     tmem_ld16x256_x2(acc + (16u << 16), *reinterpret_cast<uint32_t(*)[8]>(r + 8));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = token_scale(a, token + 8 * (j >> 1) + 2 * (lane & 3) + (j & 1));
   }
   __device__ __forceinline__ void loaded() { linear_int8::loaded(r); }
   // The channels whose scales a thread needs (of its warp's 32), and how many.
   static constexpr int kScales = 4;
   static __device__ __forceinline__ int channel(int j, int lane) { return 8 * j + (lane >> 2); }
-  __device__ __forceinline__ void put(uint32_t stage, const float (&ws)[kScales], int quarter, int sub,
+  __device__ __forceinline__ void put(uint32_t stage, float scales, const float (&ws)[kScales], int quarter, int sub,
                                       int lane) const {
+    float s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      s[j] = __shfl_sync(0xffffffffu, scales, 16 * sub + 8 * (j >> 1) + 2 * (lane & 3) + (j & 1));
     const T* t = nullptr;
     const int mat = lane >> 3, mrow = lane & 7;
     const uint32_t row =
@@ -211,21 +216,18 @@ struct Share {
 template <>
 struct Share<float> {
   uint32_t r[8];
-  float s[8];
-  __device__ __forceinline__ void load(const Args& a, uint32_t acc, int token, int) {
-    tmem_ld8(acc, r);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] = token_scale(a, token + j);
-  }
+  __device__ __forceinline__ void load(uint32_t acc) { tmem_ld8(acc, r); }
   __device__ __forceinline__ void loaded() { linear_int8::loaded(r); }
   static constexpr int kScales = 1;
   static __device__ __forceinline__ int channel(int, int lane) { return lane; }
-  __device__ __forceinline__ void put(uint32_t stage, const float (&ws)[kScales], int quarter, int sub,
+  __device__ __forceinline__ void put(uint32_t stage, float scales, const float (&ws)[kScales], int quarter, int sub,
                                       int lane) const {
-    const uint32_t at = stage + (uint32_t)(quarter * kBoxTok<float> + 8 * sub) * 128 + (uint32_t)lane * 4;
+    const uint32_t at = stage + (uint32_t)(8 * sub * kRows + quarter * 32 + lane) * 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 128u * j), "f"((float)(int)r[j] * s[j] * ws[0]) : "memory");
+    for (int j = 0; j < 8; ++j) {
+      const float v = (float)(int)r[j] * __shfl_sync(0xffffffffu, scales, 8 * sub + j) * ws[0];
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(j * kRows * 4)), "f"(v) : "memory");
+    }
   }
 };
 
@@ -233,13 +235,14 @@ struct Share<float> {
 // cannot store to.  All 32 threads of a warp.
 template <typename T>
 __device__ __forceinline__ void copy_row(const uint8_t* chunk, int i, T* y, int left, int lane) {
-  const uint8_t* box = chunk + (i / kBoxTok<T>) * (kChunkBytes / 2) + (i % kBoxTok<T>) * 128;
-  constexpr int kBoxBytes = kBoxTok<T> * 128;
   if constexpr (sizeof(T) == 4) {
+    const float* row = reinterpret_cast<const float*>(chunk) + i * kRows;
 #pragma unroll
     for (int b = 0; b < 4; ++b)
-      if (32 * b + lane < left) y[32 * b + lane] = *reinterpret_cast<const float*>(box + b * kBoxBytes + lane * 4);
+      if (32 * b + lane < left) y[32 * b + lane] = row[32 * b + lane];
   } else {
+    constexpr int kBoxBytes = kBoxTok<T> * 128;
+    const uint8_t* box = chunk + (i / kBoxTok<T>) * (kChunkBytes / 2) + (i % kBoxTok<T>) * 128;
     // Word `lane` of each box holds channels 2 lane, 2 lane + 1 (and 64 on).
     const int at = (((lane >> 2) ^ (i & 7)) << 4) + (lane & 3) * 4;
     uint32_t w[2];
@@ -318,6 +321,8 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     const int early = !a.early_w ? 0 : pre < 2 ? pre : 2;
     for (int s = 0; s < early; ++s)
       if (!stalled || s > 0) load_w(s, ks0 + s, w_row);
+    // Into L2 the weights may come at any time (a write by the kernel before would update them there).
+    for (int s = early; s < pre && s < kPrefetch; ++s) tma_prefetch_2d(&tm_w, (ks0 + s) * kBoxK, w_row, elected);
     griddep_wait();
     for (int s = 0; s < pre; ++s) {
       if (s >= early && (!stalled || s > 0)) load_w(s, ks0 + s, w_row);
@@ -423,9 +428,13 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     int iter = 0, buf_at = 0;
     uint32_t buf_round = 0;
     bool ok = true;
-    // This thread's channel scales, a tile ahead.
-    float ws_next[Share<T>::kScales];
+    // This thread's channel scales, a tile ahead, and its tokens' (one of each box) a chunk ahead.
+    float ws_next[Share<T>::kScales], s_next[2];
     int tn, tt;
+    auto request_tokens = [&](int token) {
+      s_next[0] = token_scale(a, token + lane % kBoxTok<T>);
+      s_next[1] = token_scale(a, token + kBoxTok<T> + lane % kBoxTok<T>);
+    };
     auto request = [&](int t) {
       tile_of(a, t, tn, tt);
 #pragma unroll
@@ -442,6 +451,7 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
 #pragma unroll
       for (int j = 0; j < Share<T>::kScales; ++j) ws[j] = ws_next[j];
       if (t + clusters < tiles) request(t + clusters);
+      request_tokens(token0);
       ok = waiter.wait_warp(bar(kBarAccFull + buf), (uint32_t)(iter >> 1) & 1);
       if (!ok || a.splits > 1) break;
       tc_fence_after();
@@ -461,8 +471,10 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
         const int at = c + sub * (kTok / 2);
         const bool second = c + kTok < a.tok;
         Share<T> part[2];
-        part[0].load(a, acc + (uint32_t)at, token0 + at, lane);
-        if (second) part[1].load(a, acc + (uint32_t)(at + kTok), token0 + at + kTok, lane);
+        part[0].load(acc + (uint32_t)at);
+        if (second) part[1].load(acc + (uint32_t)(at + kTok));
+        const float s0 = s_next[0], s1 = s_next[1];
+        if (c + 2 * kTok < a.tok) request_tokens(token0 + c + 2 * kTok);
         tc_wait_ld();
         part[0].loaded();
         part[1].loaded();
@@ -479,8 +491,8 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
         if (buf_round > 0) ok = waiter.wait_warp(bar(kBarChunkEmpty + buf_at), (buf_round - 1) & 1);
         if (!ok) break;
         const uint32_t stage = staging + (uint32_t)buf_at * kChunkBytes;
-        part[0].put(stage, ws, quarter, sub, lane);
-        if (second) part[1].put(stage + kChunkBytes / 2, ws, quarter, sub, lane);
+        part[0].put(stage, s0, ws, quarter, sub, lane);
+        if (second) part[1].put(stage + kChunkBytes / 2, s1, ws, quarter, sub, lane);
         if (a.tma_store) fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarChunkFull + buf_at));
@@ -699,6 +711,9 @@ int sm_count() {
   return v;
 }
 
+// Clusters of 1 to 8 CTAs that run at once on 148 SMs with one CTA each (the occupancy calculator's).
+constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+
 // Estimated microseconds of a call as waves of tiles.  A k-step takes the longest of its MMAs, the
 // shared-memory fill of a CTA and a fixed time; a tile its k-steps or, unsplit, the epilogue of the
 // tile before it; the whole at least HBM's time for the operands and y.  The constants are fitted to 1,500
@@ -708,8 +723,6 @@ int sm_count() {
 double estimate(int m, int n, int k, int group, int tok, int splits, int sms) {
   const double k_steps = (k + kBoxK - 1) / kBoxK, tiles = (double)((n + kRows * group - 1) / (kRows * group)) *
                                                           ((m + tok - 1) / tok);
-  // Clusters of 1 to 8 CTAs that run at once on 148 SMs with one CTA each (the occupancy calculator's).
-  constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
   const double slots = kClusters[group * splits] * (sms / 148.0);
   const double step = fmax(fmax(1.08 * tok, 8.06 * (16 + tok / 8.0 / group)), 157.) * 1e-3;
   const double epilogue = (5.3 * tok + 664.) * 1e-3, steps = ceil(k_steps / splits) * step;
@@ -736,6 +749,9 @@ Plan make_plan(int m, int n, int k, int sms) {
       if (i > 0 && (m <= 64 || kTokens[i - 1] >= m)) break;
       for (const int splits : kSplits) {
         if (splits * group > kMaxSplits || splits > k_steps) break;
+        // Split tiles run once each, so all at once or not at all (wq_b, 192 tiles: unsplit 8.6 us, two parts 18.6).
+        const long long tiles = (long long)((n + kRows * group - 1) / (kRows * group)) * ((m + tok - 1) / tok);
+        if (splits > 1 && tiles * 148 > (long long)kClusters[group * splits] * sms) break;
         const double t = estimate(m, n, k, group, tok, splits, sms);
         if (best.group == 0 || t < least) best = Plan{group, tok, splits, 0}, least = t;
       }
@@ -836,10 +852,11 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   if (a.stages < 1 || pl.splits > a.k_steps || pl.splits * pl.group > kMaxSplits || pl.tok > kMaxTok ||
       pl.tok % (16 * pl.group))
     return cudaErrorInvalidValue;
-  // TMA stores need rows of y on 16-byte boundaries, and write whole boxes of tokens: past a tile's end only
-  // where that is past y's end too.
+  // TMA stores need rows of y on 16-byte boundaries and write them in 16-byte units, past column n too
+  // (clipping is not by the element there), and they write whole boxes of tokens: past a tile's end
+  // only where that is past y's end.
   CUtensorMap ty = tx;
-  a.tma_store = pl.splits == 1 && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
+  a.tma_store = pl.splits == 1 && (p.n * (int64_t)sizeof(T) % 16 == 0 || (p.flags & TMLA_LINEAR_FLAG_PAD_Y)) && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
                 p.y_stride * (int64_t)sizeof(T) % 16 == 0 && encode_y<T>(&ty, p) == 0;
   const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + a.staging_bytes + kTailBytes;
   return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, stream)

@@ -162,6 +162,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
         "l"(tmap), "r"(c0), "r"(c1), "r"(bar), "l"(policy), "r"(elected)
         : "memory");
 }
+// The same tile into L2 only.
+__device__ __forceinline__ void tma_prefetch_2d(const void* tmap, int c0, int c1, uint32_t elected) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %3, 0;\n\t"
+      "@q cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];\n\t}" ::"l"(tmap),
+      "r"(c0), "r"(c1), "r"(elected)
+      : "memory");
+}
 __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t bytes, uint32_t elected) {
   asm volatile(
       "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"

@@ -168,6 +168,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_cuda(const at::Tens
                                                                   const std::optional<at::Tensor>& residual_out,
                                                                   bool overlap) {
   check_rows(x, "x");
+  TORCH_CHECK(weight.is_cuda(), "triton_mla: CUDA tensors only (there is no CPU implementation), got weight on ",
+              weight.device());
   TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(1) && weight.is_contiguous() &&
                   weight.scalar_type() == x.scalar_type() && weight.device() == x.device(),
               "triton_mla.rms_norm_int8: weight must be a contiguous [k] vector of x's dtype and device");
@@ -204,6 +206,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_meta(const at::Tens
   return {int8_rows(x), at::empty({x.size(0)}, x.options().dtype(at::kFloat)), h};
 }
 
+// y [m, n], its rows on 16-byte boundaries: the epilogue stores them by TMA.
+at::Tensor int8_product(const at::Tensor& x, const at::Tensor& w, at::ScalarType out_dtype) {
+  const int64_t m = x.size(0), n = w.size(0), per = 16 / (int64_t)at::elementSize(out_dtype);
+  return at::empty_strided({m, n}, {std::max<int64_t>(1, (n + per - 1) / per * per), 1}, x.options().dtype(out_dtype));
+}
+
 at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w,
                             const at::Tensor& w_scale, at::ScalarType out_dtype, bool overlap,
                             const std::optional<at::Tensor>& status) {
@@ -220,7 +228,7 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
   TORCH_CHECK(x.size(0) <= INT32_MAX && w.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX,
               "triton_mla.linear_int8: sizes beyond 2^31 - 1");
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor y = at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
+  at::Tensor y = int8_product(x, w, out_dtype);
   TmlaLinearInt8Params p = {};
   p.x = x.data_ptr();
   p.x_stride = row_stride(x);
@@ -229,19 +237,19 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
   p.w_stride = row_stride(w);
   p.w_scale = w_scale.data_ptr<float>();
   p.y = y.data_ptr();
-  p.y_stride = w.size(0);
+  p.y_stride = y.stride(0);
   p.m = (int32_t)x.size(0);
   p.n = (int32_t)w.size(0);
   p.k = (int32_t)x.size(1);
   p.dtype = dtype_code(out_dtype);
   p.status = status.has_value() ? status->data_ptr<int32_t>() : nullptr;
-  p.flags = overlap ? TMLA_LAYER_FLAG_PDL : 0;
+  p.flags = (overlap ? TMLA_LAYER_FLAG_PDL : 0) | TMLA_LINEAR_FLAG_PAD_Y;
   check_rc(tmla_linear_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), "tmla_linear_int8");
   return y;
 }
 at::Tensor linear_int8_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
                             at::ScalarType out_dtype, bool, const std::optional<at::Tensor>&) {
-  return at::empty({x.size(0), w.size(0)}, x.options().dtype(out_dtype));
+  return int8_product(x, w, out_dtype);
 }
 
 // Shapes only: out and lse are written in place, so there is nothing to return.

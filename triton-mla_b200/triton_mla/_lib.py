@@ -28,6 +28,7 @@ LAYER_FLAG_PDL = 1
 LINEAR_FLAG_TEST_STALL = 0x100
 LINEAR_MAX_TILES = 65536
 LINEAR_INT8_MAX_K = 131071
+LINEAR_FLAG_PAD_Y = 0x2
 W_NK = 0
 W_KN = 1
 KV_SAME = 0

@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernel import _DTYPE_CODES, _require_cuda, _status_word
+from .kernel import _DTYPE_CODES, _require_cuda, _status, _status_word
 
 
 def _stream(t: torch.Tensor):
@@ -220,12 +220,47 @@ def l2_prefetch(t: torch.Tensor, chunk_bytes: int = None, stride_bytes: int = No
 
 
 # ----------------------------------------------------------------------------- int8 projections
-def _int8_source(x: torch.Tensor) -> None:
+# The operators check their arguments themselves; these helpers name what is wrong with a refused call
+# in the package's own terms (a call that is accepted pays nothing for them: 9.5 -> 7 us of host
+# time per call).
+def _check_int8_source(x: torch.Tensor) -> None:
     _require_cuda(x)
-    assert x.dim() == 2 and x.shape[1] > 0, "a matrix [m, k] with k >= 1"
-    assert x.stride(1) == 1 or x.shape[1] == 1, "rows need unit inner stride"
     if x.dtype not in _DTYPE_CODES:
         raise TypeError(f"unsupported dtype {x.dtype}; use bfloat16, float16 or float32")
+    assert x.dim() == 2 and x.shape[1] > 0, "a matrix [m, k] with k >= 1"
+    assert x.stride(1) == 1, "rows need unit inner stride"
+
+
+def _check_rms_norm_int8(x, weight, residual, residual_out) -> None:
+    _check_int8_source(x)
+    _require_cuda(weight, residual, residual_out)
+    assert weight.shape == (x.shape[1],) and weight.dtype == x.dtype and weight.is_contiguous()
+    assert weight.device == x.device
+    for t in (residual, residual_out):
+        if t is not None:
+            assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device and t.stride(1) == 1
+    assert residual is not None or residual_out is None, "residual_out without a residual"
+
+
+def _check_linear_int8(x_q, x_scale, w_q, w_scale, out_dtype) -> None:
+    _require_cuda(x_q, x_scale, w_q, w_scale)
+    assert x_q.dim() == 2 and w_q.dim() == 2 and x_q.shape[1] == w_q.shape[1] and x_q.shape[1] > 0
+    assert x_q.dtype == torch.int8 and w_q.dtype == torch.int8, "int8 operands"
+    assert x_q.stride(1) == 1 and w_q.stride(1) == 1, "rows need unit inner stride"
+    assert x_scale.shape == x_q.shape[:1] and w_scale.shape == w_q.shape[:1], "a scale per token and per channel"
+    assert x_scale.dtype == torch.float32 and w_scale.dtype == torch.float32
+    assert x_scale.is_contiguous() and w_scale.is_contiguous()
+    assert x_q.shape[1] <= _lib.LINEAR_INT8_MAX_K, "the int32 sum of a longer k can overflow"
+    if out_dtype not in _DTYPE_CODES:
+        raise TypeError(f"unsupported out_dtype {out_dtype}; use bfloat16, float16 or float32")
+
+
+def _int8_status(device):
+    """The device's status word, unless it would have to be made during a capture (in the graph's pool)."""
+    word = _status.get(device.index)
+    if word is None and device.type == "cuda" and not torch.cuda.is_current_stream_capturing():
+        word = _status_word(device)
+    return word
 
 
 def quantize_int8(x: torch.Tensor, overlap: bool = False):
@@ -236,9 +271,12 @@ def quantize_int8(x: torch.Tensor, overlap: bool = False):
     (a scale per token) and for weights [n, k] (a scale per output channel).  A row with a NaN
     or an infinity gets scale NaN and zeros.  Rows of q start on 16-byte boundaries, so q's row
     stride is k rounded up to 16 (the padding bytes are not written).  Bf16, fp16 or fp32, any
-    row stride; no gradient.  ``overlap`` as in ``q_absorb_rope``."""
-    _int8_source(x)
-    return torch.ops.triton_mla.quantize_int8(x, overlap)
+    row stride; no gradient.  ``overlap`` as in ``rms_norm_int8`` (nothing to load early here)."""
+    try:
+        return torch.ops.triton_mla.quantize_int8(x, overlap)
+    except (RuntimeError, TypeError):
+        _check_int8_source(x)
+        raise
 
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
@@ -249,19 +287,17 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
 
     ``h = x + residual`` rounded to x's dtype, ``y = h * weight / sqrt(mean(h^2) + eps)`` in fp32,
     and y's rows quantised as in ``quantize_int8``.  x [m, k] (any row stride), weight [k].  h is
-    the new residual: a new tensor, or ``residual_out``, which may be ``residual`` or ``x`` itself.
-    Without a residual h is None and x is normalised as it is.  ``overlap`` as in
-    ``q_absorb_rope`` (the preceding kernel must not write ``weight``)."""
-    _int8_source(x)
-    _require_cuda(weight, residual, residual_out)
-    assert weight.shape == (x.shape[1],) and weight.dtype == x.dtype and weight.is_contiguous()
-    assert weight.device == x.device
-    for t in (residual, residual_out):
-        if t is not None:
-            assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device
-            assert t.stride(1) == 1 or t.shape[1] == 1
-    assert residual is not None or residual_out is None, "residual_out without a residual"
-    q, scale, h = torch.ops.triton_mla.rms_norm_int8(x, weight, eps, residual, residual_out, overlap)
+    the new residual: a new tensor, or ``residual_out``, which may be ``residual`` or ``x`` itself
+    (but overlap them in no other way).  Without a residual h is None and x is normalised as it is.
+
+    The int8 operators always launch as programmatic dependents (they wait for the preceding
+    kernel before they touch memory); ``overlap`` also lets the weight loads run before that
+    kernel has ended, which must then not write ``weight``."""
+    try:
+        q, scale, h = torch.ops.triton_mla.rms_norm_int8(x, weight, eps, residual, residual_out, overlap)
+    except (RuntimeError, TypeError):
+        _check_rms_norm_int8(x, weight, residual, residual_out)
+        raise
     if residual is None:
         return q, scale, None
     return q, scale, (h if residual_out is None else residual_out)
@@ -273,14 +309,13 @@ def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_s
     with fp32 scales per token and per output channel, as ``quantize_int8`` and ``rms_norm_int8``
     give them (C ABI: ``tmla_linear_int8``).  The products are summed exactly (int32, k at most
     131071) and scaled in fp32; y [m, n] is rounded once to ``out_dtype`` (bf16, fp16 or fp32).
-    Any m and n.  ``overlap`` as in ``linear`` (the preceding kernel must not write ``w_q``)."""
-    _require_cuda(x_q, x_scale, w_q, w_scale)
-    assert x_q.dim() == 2 and w_q.dim() == 2 and x_q.shape[1] == w_q.shape[1] and x_q.shape[1] > 0
-    assert x_q.dtype == torch.int8 and w_q.dtype == torch.int8, "int8 operands"
-    assert x_scale.shape == x_q.shape[:1] and w_scale.shape == w_q.shape[:1], "a scale per token and per channel"
-    assert x_scale.dtype == torch.float32 and w_scale.dtype == torch.float32
-    assert x_q.shape[1] <= _lib.LINEAR_INT8_MAX_K, "the int32 sum of a longer k can overflow"
-    if out_dtype not in _DTYPE_CODES:
-        raise TypeError(f"unsupported out_dtype {out_dtype}; use bfloat16, float16 or float32")
-    status = None if torch.compiler.is_compiling() else _status_word(x_q.device)
-    return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap, status)
+    Any m and n; no gradient.  Rows of y start on 16-byte boundaries (y is contiguous when a row
+    is a multiple of 16 bytes).  Rows of x_q and w_q on 16-byte boundaries run on the tcgen05
+    kernel, others on a much slower CUDA-core kernel with the same results.  ``overlap`` as in
+    ``rms_norm_int8`` (the preceding kernel must not write ``w_q``)."""
+    status = None if torch.compiler.is_compiling() else _int8_status(x_q.device)
+    try:
+        return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap, status)
+    except (RuntimeError, TypeError):
+        _check_linear_int8(x_q, x_scale, w_q, w_scale, out_dtype)
+        raise
