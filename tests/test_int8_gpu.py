@@ -303,6 +303,33 @@ def test_linear_int8_refuses_bad_operands(device):
                                 residual_out=torch.zeros(4, 8, device=device))
 
 
+def test_offsets_beyond_32_bits(device):
+    """Rows and outputs past 2^31 elements: the last rows equal those of a call on them alone."""
+    g = _gen(device, 40)
+    m, k = 140001, 16384                                   # 2.3e9 values
+    x = torch.randn(64, k, generator=g, device=device).to(torch.bfloat16).repeat(m // 64 + 1, 1)[:m]
+    x[-5:] = torch.randn(5, k, generator=g, device=device).to(torch.bfloat16)
+    w = torch.ones(k, device=device, dtype=torch.bfloat16)
+    for call in (lambda t: layer_ops.quantize_int8(t), lambda t: layer_ops.rms_norm_int8(t, w, residual=t)):
+        got, want = call(x), call(x[-5:].contiguous())
+        for a, b in zip(got, want):
+            assert torch.equal(a[-5:], b)
+        del got
+    q, s = layer_ops.quantize_int8(x[-5:, :128].contiguous())
+    xq = q.repeat(14001, 1)                                # 70005 tokens x 33000 channels: 2.3e9 products
+    wq, ws = _int8(33000, 128, g, device), torch.rand(33000, generator=g, device=device)
+    y = layer_ops.linear_int8(xq, s.repeat(14001), wq, ws)
+    _compare_linear(y[-5:], q, s, wq, ws)
+    _compare_linear(y[:5], q, s, wq, ws)
+    wide = torch.zeros(20, (1 << 27) + 16, dtype=torch.int8, device=device)   # rows 2^27 apart: 2.7e9 bytes
+    wide[:, :128] = wq[:20]
+    _compare_linear(layer_ops.linear_int8(q, s, wide[:, :128], ws[:20]), q, s, wq[:20], ws[:20])
+    _compare_linear(layer_ops.linear_int8(wide[:, :128], ws[:20], q, s), wq[:20], ws[:20], q, s)
+    odd = wide.view(-1)[: 19 * ((1 << 27) + 15) + 128].as_strided((20, 128), ((1 << 27) + 15, 1))
+    odd.copy_(wq[:20])
+    _compare_linear(layer_ops.linear_int8(q, s, odd, ws[:20]), q, s, wq[:20], ws[:20])
+
+
 # ----------------------------------------------------------------------------- used together
 class _Layer:
     """An MLA layer's decode step with int8 projections: the operators as a serving loop uses them."""
@@ -406,6 +433,40 @@ def test_two_graphs_and_two_streams_at_once(device):
             assert torch.equal(y, want)
             y.zero_()
         torch.cuda.synchronize()
+
+
+def test_calls_on_another_stream(device):
+    """The operators run on the current stream, and wait there for what came before on it."""
+    g = _gen(device, 33)
+    x = torch.randn(300, 7168, generator=g, device=device).to(torch.bfloat16)
+    w = torch.ones(7168, device=device, dtype=torch.bfloat16)
+    wq, ws = layer_ops.quantize_int8(torch.randn(512, 7168, generator=g, device=device))
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    late = torch.zeros_like(x)
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)          # about 10 ms before x is there
+        late.copy_(x)
+        q, s, h = layer_ops.rms_norm_int8(late, w, residual=late, overlap=True)
+        y = layer_ops.linear_int8(q, s, wq, ws, overlap=True)
+    stream.synchronize()
+    want = layer_ops.rms_norm_int8(x, w, residual=x)
+    assert torch.equal(q, want[0]) and torch.equal(s, want[1]) and torch.equal(h, want[2])
+    assert torch.equal(y, layer_ops.linear_int8(want[0], want[1], wq, ws))
+
+
+def test_a_weight_written_just_before(device):
+    """Without ``overlap`` the kernel before may write the weight (it is quantised in the same stream)."""
+    g = _gen(device, 34)
+    x, s = _int8(16, 4096, g, device), torch.rand(16, generator=g, device=device)
+    for i in range(10):
+        w = torch.randn(2048, 4096, generator=g, device=device).to(torch.bfloat16)
+        torch.cuda.synchronize()
+        wq, ws = layer_ops.quantize_int8(w)
+        y = layer_ops.linear_int8(x, s, wq, ws)
+        torch.cuda.synchronize()
+        assert torch.equal(y, layer_ops.linear_int8(x, s, wq, ws))
+        _compare_linear(y, x, s, wq, ws)
 
 
 def test_no_gradient_passes(device):

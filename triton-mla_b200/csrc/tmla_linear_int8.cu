@@ -388,6 +388,7 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   } else if (warp == 1) {
     // The whole warp runs this (its operands stay warp-uniform); one thread issues.
     if (leader) {
+      griddep_wait();  // a bounded wait below must not count the time of the kernel before
       const uint32_t idesc = idesc_i8(kRows * kGroup, (uint32_t)a.tok);
       const uint16_t mask = (uint16_t)(3u << (rank - half));
       int iter = 0, s = 0;
