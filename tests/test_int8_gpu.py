@@ -225,6 +225,31 @@ def test_linear_int8_matches_the_exact_product(device, m, n, k):
     assert read_status(device) == 0
 
 
+# A small case of every variant (tile of tokens, CTA pairs, parts of k) that the library chooses.
+VARIANT_SHAPES = [
+    (1, 70, 66), (1, 70, 139), (1, 85, 310), (1, 71, 404), (1, 65, 681), (19, 78, 76), (21, 69, 156), (17, 66, 292),
+    (17, 65, 439), (18, 65, 1121), (44, 64, 79), (40, 5838, 12765), (40, 4550, 2321), (41, 67, 858), (44, 92, 677),
+    (51, 75, 74), (1523, 135, 1734), (1103, 147, 1500), (74, 1414, 1222), (49, 67, 1157), (71, 9878, 77),
+    (3080, 182, 3812), (202, 1523, 4986), (380, 917, 3195), (1043, 182, 4287), (105, 9757, 90), (2941, 290, 6897),
+    (505, 1296, 4805), (1313, 344, 9712), (1246, 158, 14382), (4966, 407, 71), (2667, 313, 12568), (528, 1362, 15008),
+    (399, 15588, 75), (3801, 275, 12575), (4528, 73, 2924), (477, 846, 5464), (1321, 158, 8761), (803, 131, 14700),
+    (5063, 139, 2436), (2507, 132, 5683), (1631, 136, 7367), (1211, 143, 15211), (3837, 438, 1311), (200, 3236, 7638),
+    (1196, 391, 5139), (329, 1089, 14376), (1071, 2197, 956), (328, 3284, 10333), (540, 1702, 9208),
+    (571, 1145, 15420), (1542, 2228, 1025), (1153, 1023, 12191),
+]
+
+
+@pytest.mark.parametrize("m,n,k", VARIANT_SHAPES)
+def test_linear_int8_variants(device, m, n, k):
+    g = _gen(device, m + n + k)
+    xq, wq = _int8(m, k, g, device), _int8(n, k, g, device)
+    xs = torch.rand(m, generator=g, device=device) * 0.01 + 1e-3
+    ws = torch.rand(n, generator=g, device=device) * 1e-3 + 1e-5
+    for dtype in DTYPES:
+        _check_linear(xq, xs, wq, ws, dtype)
+    assert read_status(device) == 0
+
+
 @pytest.mark.parametrize("m,n,k,pad", [(5, 40, 100, 1), (70, 130, 257, 0), (16, 300, 1001, 2), (300, 65, 80, 3)])
 def test_linear_int8_rows_of_any_alignment(device, m, n, k, pad):
     """Rows that do not start on 16-byte boundaries (x, w or both) give the same values."""

@@ -25,6 +25,8 @@
 #include <cudaTypedefs.h>
 #include <math.h>
 
+#include <atomic>
+
 #include "tmla_common.cuh"
 #include "tmla_ptx.cuh"
 
@@ -705,13 +707,6 @@ int staging_bytes(const Plan& p) {
   return p.splits == 1 ? (int)kStagingBytes : (p.splits - 1) * ((p.tok / 4 + p.splits - 1) / p.splits) * kRows * 16;
 }
 
-int sm_count() {
-  int dev = 0, v = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return -1;
-  return v;
-}
-
 // Clusters of 1 to 8 CTAs that run at once on 148 SMs with one CTA each (the occupancy calculator's).
 constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
@@ -798,10 +793,16 @@ int encode_y(CUtensorMap* map, const TmlaLinearInt8Params& p) {
 
 template <typename T, int kGroup>
 cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtensorMap& ty, const Args& a, int clusters,
-                      size_t smem, cudaStream_t stream) {
-  cudaError_t e =
-      cudaFuncSetAttribute(int8_kernel<T, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
-  if (e != cudaSuccess) return e;
+                      size_t smem, int device, cudaStream_t stream) {
+  // The kernel's shared-memory limit is raised once on each device.
+  static std::atomic<uint64_t> raised{0};
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(raised.load(std::memory_order_relaxed) & bit)) {
+    cudaError_t e =
+        cudaFuncSetAttribute(int8_kernel<T, kGroup>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax);
+    if (e != cudaSuccess) return e;
+    if (device < 64) raised.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   const int size = kGroup * a.splits;
@@ -821,7 +822,7 @@ cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtens
 
 template <typename T>
 cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensorMap& tw, const CUtensorMap& tx, int sms,
-                   cudaStream_t stream) {
+                   int device, cudaStream_t stream) {
   Args a;
   a.m = p.m;
   a.n = p.n;
@@ -860,8 +861,8 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   a.tma_store = pl.splits == 1 && (p.n * (int64_t)sizeof(T) % 16 == 0 || (p.flags & TMLA_LINEAR_FLAG_PAD_Y)) && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
                 p.y_stride * (int64_t)sizeof(T) % 16 == 0 && encode_y<T>(&ty, p) == 0;
   const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + a.staging_bytes + kTailBytes;
-  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, stream)
-                       : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, stream);
+  return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, device, stream)
+                       : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, device, stream);
 }
 
 int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
@@ -882,17 +883,19 @@ int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
       default: e = launch_generic<float>(a, stream); break;
     }
   } else {
-    const int sms = sm_count();
-    if (sms < 1) return record_cuda_error(cudaGetLastError());
+    int device = 0, sms = 0;
+    e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return record_cuda_error(e);
     const Plan pl = make_plan(p.m, p.n, p.k, sms);
     CUtensorMap tw, tx;
     int rc = encode(&tw, p.w, p.k, p.n, p.w_stride, kRows);
     if (!rc) rc = encode(&tx, p.x, p.k, p.m, p.x_stride, pl.tok / pl.group);
     if (rc) return rc;
     switch (p.dtype) {
-      case TMLA_DTYPE_BF16: e = launch<__nv_bfloat16>(p, pl, tw, tx, sms, stream); break;
-      case TMLA_DTYPE_FP16: e = launch<__half>(p, pl, tw, tx, sms, stream); break;
-      default: e = launch<float>(p, pl, tw, tx, sms, stream); break;
+      case TMLA_DTYPE_BF16: e = launch<__nv_bfloat16>(p, pl, tw, tx, sms, device, stream); break;
+      case TMLA_DTYPE_FP16: e = launch<__half>(p, pl, tw, tx, sms, device, stream); break;
+      default: e = launch<float>(p, pl, tw, tx, sms, device, stream); break;
     }
   }
   if (e == cudaSuccess) e = cudaGetLastError();
