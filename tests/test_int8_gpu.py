@@ -225,17 +225,21 @@ def test_linear_int8_matches_the_exact_product(device, m, n, k):
     assert read_status(device) == 0
 
 
-# A small case of every variant (tile of tokens, CTA pairs, parts of k) that the library chooses.
+# A small case of every variant (tile of tokens, CTA pairs, parts of k) that the library chooses, then of
+# several tiles in a row for each that is not split.
 VARIANT_SHAPES = [
-    (1, 70, 66), (1, 70, 139), (1, 85, 310), (1, 71, 404), (1, 65, 681), (19, 78, 76), (21, 69, 156), (17, 66, 292),
-    (17, 65, 439), (18, 65, 1121), (44, 64, 79), (40, 5838, 12765), (40, 4550, 2321), (41, 67, 858), (44, 92, 677),
-    (51, 75, 74), (1523, 135, 1734), (1103, 147, 1500), (74, 1414, 1222), (49, 67, 1157), (71, 9878, 77),
-    (3080, 182, 3812), (202, 1523, 4986), (380, 917, 3195), (1043, 182, 4287), (105, 9757, 90), (2941, 290, 6897),
-    (505, 1296, 4805), (1313, 344, 9712), (1246, 158, 14382), (4966, 407, 71), (2667, 313, 12568), (528, 1362, 15008),
-    (399, 15588, 75), (3801, 275, 12575), (4528, 73, 2924), (477, 846, 5464), (1321, 158, 8761), (803, 131, 14700),
-    (5063, 139, 2436), (2507, 132, 5683), (1631, 136, 7367), (1211, 143, 15211), (3837, 438, 1311), (200, 3236, 7638),
-    (1196, 391, 5139), (329, 1089, 14376), (1071, 2197, 956), (328, 3284, 10333), (540, 1702, 9208),
-    (571, 1145, 15420), (1542, 2228, 1025), (1153, 1023, 12191),
+    (1, 70, 66), (1, 5833, 937), (1, 2855, 667), (1, 66, 827), (1, 65, 681), (17, 64, 80), (17, 5963, 1638),
+    (17, 3325, 1148), (18, 99, 989), (18, 65, 1121), (44, 64, 79), (37, 5769, 2271), (34, 4700, 2040),
+    (42, 2945, 1622), (44, 64, 1827), (51, 75, 74), (65, 3931, 2697), (1060, 146, 2342), (712, 131, 2235),
+    (49, 75, 1891), (72, 9497, 65), (5289, 81, 5243), (73, 4844, 4039), (74, 2823, 4174), (76, 2069, 5969),
+    (105, 9757, 90), (7899, 70, 9850), (4994, 76, 6213), (3247, 72, 14278), (2429, 73, 14496), (4966, 407, 71),
+    (1441, 629, 15498), (6130, 66, 15315), (399, 15588, 75), (18, 19036, 2456), (18, 7076, 14510),
+    (2890, 69, 2424), (1670, 141, 4846), (1074, 138, 10210), (857, 140, 9719), (66, 22254, 805),
+    (71, 6052, 5598), (71, 4585, 6483), (79, 2927, 6359), (110, 11256, 1156), (3873, 147, 9519),
+    (2507, 132, 5683), (1571, 156, 12675), (133, 10819, 984), (5949, 162, 13338), (3260, 147, 16124),
+    (163, 3096, 14149), (215, 10039, 940), (4839, 157, 15228), (123, 21038, 72), (285, 13500, 64),
+    (223, 23140, 77), (1070, 8540, 65), (644, 18176, 65), (168, 20370, 576), (198, 19026, 669),
+    (525, 12991, 656), (653, 17786, 520),
 ]
 
 

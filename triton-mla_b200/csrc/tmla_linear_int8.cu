@@ -53,7 +53,7 @@ constexpr int kThreads = 32 * (kStoreWarp + 1);
 // y leaves in chunks of 128 channels x 2 kBoxTok<T> tokens, staged in shared memory as boxes of
 // kBoxChannels<T> channels (128 bytes of 16-bit values, swizzled; all 128 of fp32) x kBoxTok<T> tokens.
 constexpr uint32_t kChunkBytes = 16384;
-constexpr int kChunkBufs = 2;
+constexpr int kChunkBufs = 3;
 constexpr uint32_t kStagingBytes = kChunkBufs * kChunkBytes;
 template <typename T>
 constexpr int kBoxTok = (int)(kChunkBytes / (2 * kRows * sizeof(T)));  // 32 of 16 bits, 16 of fp32
@@ -560,10 +560,10 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
     }
     __syncwarp();
   } else if (a.tma_store) {
-    // The store warp: a staged chunk to y by TMA, and its buffer back once it has been read.
+    // The store warp: a staged chunk to y by TMA, and the buffer of the chunk before back, which has been read.
     constexpr int kTok = kBoxTok<T>;
     griddep_wait();
-    int at = 0;
+    int at = 0, before = -1;
     uint32_t phase = 0;
     bool ok = true;
     for (int t = cluster; t < tiles && ok; t += clusters) {
@@ -587,10 +587,11 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
         }
         if (elected) {
           bulk_commit_group();
-          bulk_wait_group_read<0>();
-          mbar_arrive(bar(kBarChunkEmpty + at));
+          bulk_wait_group_read<1>();
+          if (before >= 0) mbar_arrive(bar(kBarChunkEmpty + before));
         }
         __syncwarp();
+        before = at;
         if (++at == kChunkBufs) at = 0, phase ^= 1;
       }
     }
@@ -710,30 +711,31 @@ int staging_bytes(const Plan& p) {
 // Clusters of 1 to 8 CTAs that run at once on 148 SMs with one CTA each (the occupancy calculator's).
 constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
-// Estimated microseconds of a call as waves of tiles.  A k-step takes the longest of its MMAs, the
-// shared-memory fill of a CTA and a fixed time; a tile its k-steps or, unsplit, the epilogue of the
-// tile before it; the whole at least HBM's time for the operands and y.  The constants are fitted to 1,500
-// calls measured on B200 (1 to 4096 tokens, eight n x k from 512 x 16384 to 20000 x 128, all variants,
-// bf16 out): the variant with the least estimate is on average 1.4% slower than the fastest measured,
-// 11% at worst.
-double estimate(int m, int n, int k, int group, int tok, int splits, int sms) {
+// Estimated microseconds of a call, up to a constant.  The tiles run in waves; a k-step of a tile takes the
+// longer of its MMAs and the fill of a CTA's shared memory, an unsplit tile at least the epilogue of the tile
+// before it.  HBM's time for the operands and y overlaps in part.  The constants are fitted to 2,300
+// calls measured on B200 (1 to 8000 tokens, twelve n x k from 300 x 300 to 512 x 16384 and 24576 x 1536, every
+// variant, bf16 out): the variant with the least estimate is on average 1.8% slower than the fastest
+// measured, 17% at worst.
+double estimate(int m, int n, int k, int size, int group, int tok, int splits, int sms) {
   const double k_steps = (k + kBoxK - 1) / kBoxK, tiles = (double)((n + kRows * group - 1) / (kRows * group)) *
                                                           ((m + tok - 1) / tok);
   const double slots = kClusters[group * splits] * (sms / 148.0);
-  const double step = fmax(fmax(1.08 * tok, 8.06 * (16 + tok / 8.0 / group)), 157.) * 1e-3;
-  const double epilogue = (5.3 * tok + 664.) * 1e-3, steps = ceil(k_steps / splits) * step;
+  const double step = fmax(fmax(0.986 * tok, 7.773 * (16 + tok / 8.0 / group)), 60.6) * 1e-3;
+  const double epilogue = (4.286 * tok + 418.) * 1e-3, steps = ceil(k_steps / splits) * step;
   const double tiles_us = ceil(tiles / slots) * (splits == 1 ? fmax(steps, epilogue) : steps);
-  const double hbm_us = ((double)n * k + (double)m * k + 1.8 * m * n) / 4.25e6;
-  return (group == 2 ? 0.69 : 0.) + fmax(tiles_us, hbm_us) + 0.11 * fmin(tiles_us, hbm_us) +
-         (splits == 1 ? epilogue : 0.36 + 0.029 * tok);
+  const double hbm_us = ((double)n * k + (double)m * k + 1.764 * size * m * n) / 9.67e6;
+  return (group == 2 ? 0.589 : 0.) + fmax(tiles_us, hbm_us) + 0.723 * fmin(tiles_us, hbm_us) +
+         (splits == 1 ? epilogue : 0.366 + 0.035 * tok);
 }
 
-// The variant with the least estimate.  Examples (us measured, chosen against the next kind):
-//   16 tokens, wo (7168 x 16384): 2 parts 23.9, unsplit 24.5, CTA pairs 24.8;
-//   16 tokens, [wq_a; wkv_a] (2112 x 7168): 6 parts 6.9, unsplit 10.4;
-//   256 tokens, wo: pairs of 128 tokens 32.0, single CTAs 33.9;  4096 tokens, wq_b: pairs of 256 113, single 122;
-//   4096 tokens, 20000 x 128: single CTAs 50, pairs 58.
-Plan make_plan(int m, int n, int k, int sms) {
+// The variant with the least estimate.  Examples (us measured, the chosen one first):
+//   wo (7168 x 16384), 16 tokens: 2 parts 23.1, unsplit 25.1;  64 tokens: pairs in 2 parts 24.6, single
+//   CTAs in 2 parts 25.6, pairs unsplit 27.8;  256 tokens: pairs of 128 33.7, single CTAs of 128 37.3, pairs of
+//   256 in 2 parts 36.9;  [wq_a; wkv_a] (2112 x 7168), 16 tokens: 6 parts 6.6, unsplit 10.3;
+//   wq_b (24576 x 1536), 4096 tokens: pairs of 256 109, single CTAs 131;
+//   20000 x 128, 4096 tokens: single CTAs 48, pairs 57.
+Plan make_plan(int m, int n, int k, int size, int sms) {
   constexpr int kTokens[] = {64, 96, 128, 192, 256}, kSplits[] = {1, 2, 3, 4, 6};
   Plan best{};
   double least = 0;
@@ -748,7 +750,7 @@ Plan make_plan(int m, int n, int k, int sms) {
         // Split tiles run once each, so all at once or not at all (wq_b, 192 tiles: unsplit 8.6 us, two parts 18.6).
         const long long tiles = (long long)((n + kRows * group - 1) / (kRows * group)) * ((m + tok - 1) / tok);
         if (splits > 1 && tiles * 148 > (long long)kClusters[group * splits] * sms) break;
-        const double t = estimate(m, n, k, group, tok, splits, sms);
+        const double t = estimate(m, n, k, size, group, tok, splits, sms);
         if (best.group == 0 || t < least) best = Plan{group, tok, splits, 0}, least = t;
       }
     }
@@ -887,7 +889,7 @@ int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
     e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return record_cuda_error(e);
-    const Plan pl = make_plan(p.m, p.n, p.k, sms);
+    const Plan pl = make_plan(p.m, p.n, p.k, p.dtype == TMLA_DTYPE_FP32 ? 4 : 2, sms);
     CUtensorMap tw, tx;
     int rc = encode(&tw, p.w, p.k, p.n, p.w_stride, kRows);
     if (!rc) rc = encode(&tx, p.x, p.k, p.m, p.x_stride, pl.tok / pl.group);
