@@ -104,15 +104,16 @@ void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& le
 // ---------------------------------------------------------------- int8 projections
 // quantize_int8(x [m, k]) -> (q int8 [m, k], scale fp32 [m]); rms_norm_int8 -> (q, scale, h): h is a
 // new tensor when there is a residual and no residual_out, else empty; linear_int8(x_q [m, k],
-// x_scale [m], w_q [n, k], w_scale [n]) -> y [m, n] in out_dtype.  Rows of q start on 16-byte
-// boundaries (row stride k rounded up to 16), as linear_int8's TMA loads want them.  Outputs come
+// x_scale [m], w_q [n, k], w_scale [n]) -> y [m, n] in out_dtype.  Rows of q, h and y start on 16-byte
+// boundaries (a row stride of k or n rounded up), as the kernels' vector accesses and TMA want them.  Outputs come
 // from the caching allocator, the launches go on the current stream of the inputs' device.
 
-// An [m, k] int8 tensor whose rows start on 16-byte boundaries.
-at::Tensor int8_rows(const at::Tensor& x) {
-  const int64_t m = x.size(0), k = x.size(1), stride = (k + 15) / 16 * 16;
-  return at::empty_strided({m, k}, {stride, 1}, x.options().dtype(at::kChar));
+// An [m, n] tensor whose rows start on 16-byte boundaries.
+at::Tensor aligned_rows(int64_t m, int64_t n, const at::TensorOptions& options, at::ScalarType dtype) {
+  const int64_t per = 16 / (int64_t)at::elementSize(dtype);
+  return at::empty_strided({m, n}, {std::max<int64_t>(1, (n + per - 1) / per * per), 1}, options.dtype(dtype));
 }
+at::Tensor int8_rows(const at::Tensor& x) { return aligned_rows(x.size(0), x.size(1), x.options(), at::kChar); }
 
 void check_rows(const at::Tensor& t, const char* what) {
   TORCH_CHECK(t.is_cuda(), "triton_mla: CUDA tensors only (there is no CPU implementation), got ", what, " on ",
@@ -185,7 +186,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_cuda(const at::Tens
     if (residual_out.has_value())
       check_like(*residual_out, x, "residual_out");
     else
-      h = at::empty({x.size(0), x.size(1)}, x.options());
+      h = aligned_rows(x.size(0), x.size(1), x.options(), x.scalar_type());
     const at::Tensor& out = residual_out.has_value() ? *residual_out : h;
     p.residual = residual->data_ptr();
     p.residual_stride = row_stride(*residual);
@@ -201,15 +202,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_meta(const at::Tens
                                                                   const std::optional<at::Tensor>& residual,
                                                                   const std::optional<at::Tensor>& residual_out,
                                                                   bool) {
-  at::Tensor h = residual.has_value() && !residual_out.has_value() ? at::empty({x.size(0), x.size(1)}, x.options())
-                                                                   : at::empty({0}, x.options());
+  at::Tensor h = residual.has_value() && !residual_out.has_value()
+                     ? aligned_rows(x.size(0), x.size(1), x.options(), x.scalar_type())
+                     : at::empty({0}, x.options());
   return {int8_rows(x), at::empty({x.size(0)}, x.options().dtype(at::kFloat)), h};
-}
-
-// y [m, n], its rows on 16-byte boundaries: the epilogue stores them by TMA.
-at::Tensor int8_product(const at::Tensor& x, const at::Tensor& w, at::ScalarType out_dtype) {
-  const int64_t m = x.size(0), n = w.size(0), per = 16 / (int64_t)at::elementSize(out_dtype);
-  return at::empty_strided({m, n}, {std::max<int64_t>(1, (n + per - 1) / per * per), 1}, x.options().dtype(out_dtype));
 }
 
 at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w,
@@ -228,7 +224,7 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
   TORCH_CHECK(x.size(0) <= INT32_MAX && w.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX,
               "triton_mla.linear_int8: sizes beyond 2^31 - 1");
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor y = int8_product(x, w, out_dtype);
+  at::Tensor y = aligned_rows(x.size(0), w.size(0), x.options(), out_dtype);
   TmlaLinearInt8Params p = {};
   p.x = x.data_ptr();
   p.x_stride = row_stride(x);
@@ -249,7 +245,7 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
 }
 at::Tensor linear_int8_meta(const at::Tensor& x, const at::Tensor&, const at::Tensor& w, const at::Tensor&,
                             at::ScalarType out_dtype, bool, const std::optional<at::Tensor>&) {
-  return int8_product(x, w, out_dtype);
+  return aligned_rows(x.size(0), w.size(0), x.options(), out_dtype);
 }
 
 // Shapes only: out and lse are written in place, so there is nothing to return.
