@@ -167,6 +167,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// (a0 b0 c, a1 b1 c) as two packed products.
+__device__ __forceinline__ float2 scale2(float a0, float a1, float2 b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %6};\n\t"
+      "mul.rn.f32x2 a, a, b;\n\tmul.rn.f32x2 a, a, c;\n\t"
+      "mov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a0), "f"(a1), "f"(b.x), "f"(b.y), "f"(c));
+  return r;
+}
+
 // Past a wait for TMEM loads: their registers are read after it.
 template <int N>
 __device__ __forceinline__ void loaded(uint32_t (&r)[N]) {
@@ -206,9 +218,11 @@ struct Share {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t* q = r + 8 * h + 4 * j;
-        v[2 * j] = pack2((float)(int)q[0] * s[2 * j] * ws[2 * h], (float)(int)q[1] * s[2 * j + 1] * ws[2 * h], t);
-        v[2 * j + 1] =
-            pack2((float)(int)q[2] * s[2 * j] * ws[2 * h + 1], (float)(int)q[3] * s[2 * j + 1] * ws[2 * h + 1], t);
+        const float2 st = make_float2(s[2 * j], s[2 * j + 1]);
+        const float2 lo = scale2((float)(int)q[0], (float)(int)q[1], st, ws[2 * h]);
+        const float2 hi = scale2((float)(int)q[2], (float)(int)q[3], st, ws[2 * h + 1]);
+        v[2 * j] = pack2(lo.x, lo.y, t);
+        v[2 * j + 1] = pack2(hi.x, hi.y, t);
       }
       const uint32_t chunk16 = (uint32_t)((quarter & 1) * 4 + h * 2 + (mat & 1));
       stmatrix_x4_trans(row + ((chunk16 ^ (uint32_t)mrow) << 4), v[0], v[1], v[2], v[3]);
@@ -226,9 +240,12 @@ struct Share<float> {
                                       int lane) const {
     const uint32_t at = stage + (uint32_t)(8 * sub * kRows + quarter * 32 + lane) * 4;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = (float)(int)r[j] * __shfl_sync(0xffffffffu, scales, 8 * sub + j) * ws[0];
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(j * kRows * 4)), "f"(v) : "memory");
+    for (int j = 0; j < 8; j += 2) {
+      const float2 s = make_float2(__shfl_sync(0xffffffffu, scales, 8 * sub + j),
+                                   __shfl_sync(0xffffffffu, scales, 8 * sub + j + 1));
+      const float2 v = scale2((float)(int)r[j], (float)(int)r[j + 1], s, ws[0]);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(j * kRows * 4)), "f"(v.x) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)((j + 1) * kRows * 4)), "f"(v.y) : "memory");
     }
   }
 };
