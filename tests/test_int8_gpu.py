@@ -229,17 +229,21 @@ def test_linear_int8_matches_the_exact_product(device, m, n, k):
 # several tiles in a row for each that is not split.
 VARIANT_SHAPES = [
     (1, 70, 66), (1, 5833, 937), (1, 2855, 667), (1, 66, 827), (1, 65, 681), (17, 64, 80), (17, 5963, 1638),
-    (17, 3325, 1148), (18, 99, 989), (18, 65, 1121), (44, 64, 79), (37, 5769, 2271), (34, 4700, 2040),
-    (42, 2945, 1622), (44, 64, 1827), (51, 75, 74), (65, 3931, 2697), (1060, 146, 2342), (712, 131, 2235),
+    (17, 3325, 1148), (17, 64, 916), (18, 65, 1121), (38, 65, 69), (37, 5769, 2271), (34, 4700, 2040),
+    (42, 2945, 1622), (34, 74, 1285), (51, 75, 74), (2981, 65, 2835), (65, 2195, 2314), (712, 131, 2235),
     (49, 75, 1891), (72, 9497, 65), (5289, 81, 5243), (73, 4844, 4039), (74, 2823, 4174), (76, 2069, 5969),
-    (105, 9757, 90), (7899, 70, 9850), (4994, 76, 6213), (3247, 72, 14278), (2429, 73, 14496), (4966, 407, 71),
-    (1441, 629, 15498), (6130, 66, 15315), (399, 15588, 75), (18, 19036, 2456), (18, 7076, 14510),
-    (2890, 69, 2424), (1670, 141, 4846), (1074, 138, 10210), (857, 140, 9719), (66, 22254, 805),
-    (71, 6052, 5598), (71, 4585, 6483), (79, 2927, 6359), (110, 11256, 1156), (3873, 147, 9519),
-    (2507, 132, 5683), (1571, 156, 12675), (133, 10819, 984), (5949, 162, 13338), (3260, 147, 16124),
-    (163, 3096, 14149), (215, 10039, 940), (4839, 157, 15228), (123, 21038, 72), (285, 13500, 64),
-    (223, 23140, 77), (1070, 8540, 65), (644, 18176, 65), (168, 20370, 576), (198, 19026, 669),
-    (525, 12991, 656), (653, 17786, 520),
+    (114, 10078, 73), (7899, 70, 9850), (5265, 64, 6676), (3591, 70, 15297), (2429, 73, 14496),
+    (132, 14199, 65), (3801, 275, 12575), (7118, 78, 10075), (5155, 67, 13987), (3215, 72, 12171),
+    (483, 5081, 66), (2698, 372, 14606), (6130, 66, 15315), (5919, 582, 64), (7339, 75, 12801),
+    (1732, 5143, 69), (18, 19036, 2456), (18, 7076, 14510), (2890, 69, 2424), (1670, 141, 4846),
+    (1133, 151, 7840), (857, 140, 9719), (66, 22254, 805), (71, 6052, 5598), (1653, 130, 7935),
+    (1434, 140, 6269), (110, 11256, 1156), (3873, 147, 9519), (2507, 132, 5683), (1571, 156, 12675),
+    (133, 10819, 984), (5150, 132, 10419), (129, 4534, 10003), (155, 3097, 9051), (163, 10279, 1011),
+    (5949, 162, 13338), (3686, 149, 14130), (163, 3096, 14149), (215, 10039, 940), (2343, 537, 13253),
+    (200, 4414, 12501), (200, 2954, 13107), (242, 9811, 953), (5611, 147, 12749), (118, 20718, 76),
+    (170, 20273, 92), (223, 23140, 77), (319, 19197, 74), (1070, 8540, 65), (441, 20197, 74), (678, 16360, 74),
+    (168, 20370, 576), (193, 24380, 569), (706, 9700, 571), (357, 20186, 654), (3058, 3660, 533),
+    (4075, 2973, 517),
 ]
 
 

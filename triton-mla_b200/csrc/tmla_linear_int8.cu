@@ -3,10 +3,10 @@
 // neither the order of the terms nor the way k is cut changes the result.
 //
 // tcgen05 kernel (int8_kernel).  The weight rows (output channels) are the MMA's M and the tokens its
-// N, whatever their numbers: D[channel][token] then has one channel per TMEM lane, so that a
-// warp of the epilogue writes 32 neighbouring channels of a token at once, straight to y, and
-// one token or an odd n costs a predicate.  One instantiation serves all sizes; the token tile
-// N is an argument.
+// N, whatever their numbers: a tile is 128 channels (one TMEM lane each) x 16 to 256 tokens, so that one
+// token wastes no more than 15, and D[channel][token] leaves TMEM with neighbouring channels in
+// neighbouring lanes, as y's rows want them.  One instantiation per type serves all sizes; the
+// tile's tokens N are an argument.
 //   kGroup = 1: one CTA per tile of 128 channels.
 //   kGroup = 2: a CTA pair per tile of 256 channels (cta_group::2): each CTA holds its 128 weight
 //     rows and half of the tokens, which halves what an MMA reads of the token operand.
@@ -17,6 +17,17 @@
 // TMA into a ring of stages; warp 1 issues the MMAs (the pair's even CTA for both); warps 2-9
 // are the epilogue; warp 10 stores what they stage.  Unsplit CTAs are persistent, with two
 // accumulators, so that a tile's epilogue runs under the next tile's MMAs.
+//
+// What bounds it, and what it reaches on B200 (weights not in L2, calls back to back).  Few tokens: the weight's
+// stream from HBM.  wo (7168 x 16384) 16 tokens 22.5 us (81% of a copy's bandwidth), wq_b (24576 x 1536) 8.6 us,
+// [wq_a; wkv_a] (2112 x 7168) 6.6 us, of which a launch with nothing to do is 2.3.  Many tokens: the MMAs; wo 8192
+// tokens 600 us = 3.2e15 operations a second at the clock that 1000 W allow, the tensor pipe active for
+// 87% of the cycles of a full wave.  Small k: the epilogue; 4096 x 32768 x 512 82 us, 3.3 TB/s of y.
+//   An issuing thread alone in its branch took 66 cycles for each MMA and 100 for each TMA load (every operand
+//   moved to a uniform register), 560 a k-step whatever its size, above the MMAs' 512.  With the warp converged
+//   and one elected thread wo 8192 tokens in tiles of 128 went from 1106 to 832 us.
+//   Four epilogue warps with stores of single columns took 13 us for a pair's tile of 256 tokens; eight, with y staged
+//   and stored by TMA, 2.3.  Sixteen took as long, and a launch 1 us more.
 //
 // Every wait is bounded (2 s by default): on expiry the kernel sets TMLA_STATUS_TIMEOUT, stops,
 // drains the copies and MMAs that it issued, leaves the tiles that it could not finish unwritten,
@@ -94,8 +105,7 @@ struct Waiter {
   volatile int* abort_flag;
   int* status;
   uint64_t limit_ns;
-  // kCluster: the arrivals come from threads of another CTA (acquire at cluster scope, which costs more
-  // than the loads and MMA completions of a stage should pay).
+  // kCluster: the arrivals come from threads of another CTA.
   template <bool kCluster = false>
   __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) const {
     uint64_t t0 = 0;
@@ -186,7 +196,7 @@ __device__ __forceinline__ void loaded(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 
-// A warp's share of a box of tokens: its 32 channels x half of the tokens, from `token` and `acc` on.
+// A warp's share of a box of tokens: its 32 channels x half of the tokens.
 // 16-bit y: 16 tokens.  The 16x256b loads leave the accumulator in the registers as 8 x 8 matrices of
 // channels x tokens, which stmatrix writes transposed into 128-byte swizzled rows of 64 channels.
 // fp32 y: 8 tokens, a thread's channel straight into rows of 128 channels.
@@ -319,7 +329,7 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
   const bool stalled = a.stall && blockIdx.x == 0;
   // A weight row is used by one token tile only, or again by the next ones.
   const uint64_t pol_w = a.t_tiles == 1 ? policy_evict_first() : policy_evict_normal();
-  const uint64_t pol_x = policy_evict_last();
+  const uint64_t pol_x = policy_evict_last();  // every channel tile re-reads it (2000 x 12000 x 6000: 132 us, else 150)
   const uint32_t pair_bar = kGroup == 2 ? map_to_rank(bar(0), (uint32_t)(rank - half)) : bar(0);
   auto load_w = [&](int s, int ks, int row) {
     if (leader) mbar_arrive_expect_tx(bar(kBarFull + s), (uint32_t)(kGroup * (kWBytes + a.x_bytes)), elected);
@@ -476,16 +486,6 @@ __global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ 
       if (!ok || a.splits > 1) break;
       tc_fence_after();
       const uint32_t acc = lanes + (uint32_t)(buf * a.acc_cols);
-      auto release = [&]() {  // the accumulator has been read
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (kGroup == 2)
-            mbar_arrive_cluster(map_to_rank(bar(kBarAccEmpty + buf), (uint32_t)(rank - half)));
-          else
-            mbar_arrive(bar(kBarAccEmpty + buf));
-        }
-      };
       constexpr int kTok = kBoxTok<T>;
       for (int c = 0; c < a.tok; c += 2 * kTok) {
         const int at = c + sub * (kTok / 2);
@@ -753,12 +753,12 @@ double estimate(int m, int n, int k, int size, int group, int tok, int splits, i
 //   wq_b (24576 x 1536), 4096 tokens: pairs of 256 109, single CTAs 131;
 //   20000 x 128, 4096 tokens: single CTAs 48, pairs 57.
 Plan make_plan(int m, int n, int k, int size, int sms) {
-  constexpr int kTokens[] = {64, 96, 128, 192, 256}, kSplits[] = {1, 2, 3, 4, 6};
+  constexpr int kTokens[] = {64, 96, 128, 160, 192, 224, 256}, kSplits[] = {1, 2, 3, 4, 6};
   Plan best{};
   double least = 0;
   const int k_steps = (k + kBoxK - 1) / kBoxK;
   for (int group = 1; group <= 2; ++group) {
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 7; ++i) {
       // Up to 64 tokens one tile holds them all, in steps of the MMA's N.
       const int step = 16 * group, tok = m <= 64 ? (m + step - 1) / step * step : kTokens[i];
       if (i > 0 && (m <= 64 || kTokens[i - 1] >= m)) break;
@@ -854,6 +854,7 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   a.stages = pl.stages;
   a.stage_bytes = kRows * kBoxK + a.x_bytes;
   a.staging_bytes = staging_bytes(pl);
+  if ((long long)a.n_tiles * a.t_tiles > kMaxRows) return cudaErrorInvalidValue;  // a y beyond any memory
   const int tiles = a.n_tiles * a.t_tiles;
   const int resident = sms / pl.group;
   const int clusters = pl.splits > 1 || tiles < resident ? tiles : resident;
@@ -877,8 +878,10 @@ cudaError_t launch(const TmlaLinearInt8Params& p, const Plan& pl, const CUtensor
   // (clipping is not by the element there), and they write whole boxes of tokens: past a tile's end
   // only where that is past y's end.
   CUtensorMap ty = tx;
-  a.tma_store = pl.splits == 1 && (p.n * (int64_t)sizeof(T) % 16 == 0 || (p.flags & TMLA_LINEAR_FLAG_PAD_Y)) && (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 &&
-                p.y_stride * (int64_t)sizeof(T) % 16 == 0 && encode_y<T>(&ty, p) == 0;
+  const int64_t size = sizeof(T);
+  a.tma_store = pl.splits == 1 && (p.n * size % 16 == 0 || (p.flags & TMLA_LINEAR_FLAG_PAD_Y)) &&
+                (pl.tok % kBoxTok<T> == 0 || a.t_tiles == 1) && (uintptr_t)p.y % 16 == 0 && p.y_stride * size % 16 == 0 &&
+                encode_y<T>(&ty, p) == 0;
   const size_t smem = 1024 + (size_t)a.stages * a.stage_bytes + a.staging_bytes + kTailBytes;
   return pl.group == 1 ? launch_tc<T, 1>(tw, tx, ty, a, clusters, smem, device, stream)
                        : launch_tc<T, 2>(tw, tx, ty, a, clusters, smem, device, stream);
