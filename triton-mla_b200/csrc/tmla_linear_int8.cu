@@ -825,17 +825,17 @@ cudaError_t launch_tc(const CUtensorMap& tw, const CUtensorMap& tx, const CUtens
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   const int size = kGroup * a.splits;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)size;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)size;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(clusters * size));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = size > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, int8_kernel<T, kGroup>, tw, tx, ty, a);
 }
 
