@@ -468,6 +468,32 @@ def test_two_graphs_and_two_streams_at_once(device):
         torch.cuda.synchronize()
 
 
+def test_first_calls_inside_a_capture(device):
+    """A process whose first calls are captured: nothing has to be set up before."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    code = """
+import torch
+from triton_mla import layer_ops, read_status
+x = torch.randn(40, 512, device="cuda", dtype=torch.bfloat16)
+w = torch.ones(512, device="cuda", dtype=torch.bfloat16)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    q, s, h = layer_ops.rms_norm_int8(x, w, residual=x)
+    y = layer_ops.linear_int8(q, s, q, s, torch.float32)
+graph.replay()
+torch.cuda.synchronize()
+q2, s2, _ = layer_ops.rms_norm_int8(x, w, residual=x)
+assert torch.equal(q, q2) and torch.equal(y, layer_ops.linear_int8(q2, s2, q2, s2, torch.float32))
+assert read_status() == 0
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=ROOT / "triton-mla_b200", capture_output=True, text=True,
+                         timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
+
+
 def test_calls_on_another_stream(device):
     """The operators run on the current stream, and wait there for what came before on it."""
     g = _gen(device, 33)
@@ -508,6 +534,10 @@ def test_no_gradient_passes(device):
     q, s, h = layer_ops.rms_norm_int8(x, w, residual=x)
     assert not s.requires_grad and not h.requires_grad
     assert not layer_ops.quantize_int8(x)[1].requires_grad
+    y = torch.randn(4, 64, device=device)
+    version = y._version
+    layer_ops.rms_norm_int8(y, w.detach(), residual=y, residual_out=y)
+    assert y._version > version, "a write in place is seen by autograd"
 
 
 def test_int8_operators_compile_without_a_graph_break(device):

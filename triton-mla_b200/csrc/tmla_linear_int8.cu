@@ -27,7 +27,7 @@
 //   moved to a uniform register), 560 a k-step whatever its size, above the MMAs' 512.  With the warp converged
 //   and one elected thread wo 8192 tokens in tiles of 128 went from 1106 to 832 us.
 //   Four epilogue warps with stores of single columns took 13 us for a pair's tile of 256 tokens; eight, with y staged
-//   and stored by TMA, 2.3.  Sixteen took as long, and a launch 1 us more.
+//   and stored by TMA, 2.3.  Sixteen took as long.
 //
 // Every wait is bounded (2 s by default): on expiry the kernel sets TMLA_STATUS_TIMEOUT, stops,
 // drains the copies and MMAs that it issued, leaves the tiles that it could not finish unwritten,
@@ -299,7 +299,7 @@ __device__ __forceinline__ void copy_row(const uint8_t* chunk, int i, T* y, int 
 }
 
 template <typename T, int kGroup>
-__global__ void __launch_bounds__(kThreads) int8_kernel(const __grid_constant__ CUtensorMap tm_w,
+__global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant__ CUtensorMap tm_w,
                                                         const __grid_constant__ CUtensorMap tm_x,
                                                         const __grid_constant__ CUtensorMap tm_y, const Args a) {
   extern __shared__ uint8_t smem_raw[];

@@ -192,6 +192,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_cuda(const at::Tens
     p.residual_stride = row_stride(*residual);
     p.h = out.data_ptr();
     p.h_stride = row_stride(out);
+    // Autograd must see that a caller's tensor has been written.
+    if (residual_out.has_value() && !residual_out->is_inference())
+      residual_out->unsafeGetTensorImpl()->bump_version();
   }
   if (!h.defined()) h = at::empty({0}, x.options());
   check_rc(tmla_rms_norm_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()),
