@@ -228,22 +228,22 @@ def test_linear_int8_matches_the_exact_product(device, m, n, k):
 # A small case of every variant (tile of tokens, CTA pairs, parts of k) that the library chooses, then of
 # several tiles in a row for each that is not split.
 VARIANT_SHAPES = [
-    (1, 70, 66), (1, 5833, 937), (1, 2855, 667), (1, 66, 827), (1, 65, 681), (17, 64, 80), (17, 5963, 1638),
-    (17, 3325, 1148), (17, 64, 916), (18, 65, 1121), (38, 65, 69), (37, 5769, 2271), (34, 4700, 2040),
-    (42, 2945, 1622), (34, 74, 1285), (51, 75, 74), (2981, 65, 2835), (65, 2195, 2314), (712, 131, 2235),
-    (49, 75, 1891), (72, 9497, 65), (5289, 81, 5243), (73, 4844, 4039), (74, 2823, 4174), (76, 2069, 5969),
-    (114, 10078, 73), (7899, 70, 9850), (5265, 64, 6676), (3591, 70, 15297), (2429, 73, 14496),
-    (132, 14199, 65), (3801, 275, 12575), (7118, 78, 10075), (5155, 67, 13987), (3215, 72, 12171),
-    (483, 5081, 66), (2698, 372, 14606), (6130, 66, 15315), (5919, 582, 64), (7339, 75, 12801),
-    (1732, 5143, 69), (18, 19036, 2456), (18, 7076, 14510), (2890, 69, 2424), (1670, 141, 4846),
-    (1133, 151, 7840), (857, 140, 9719), (66, 22254, 805), (71, 6052, 5598), (1653, 130, 7935),
-    (1434, 140, 6269), (110, 11256, 1156), (3873, 147, 9519), (2507, 132, 5683), (1571, 156, 12675),
-    (133, 10819, 984), (5150, 132, 10419), (129, 4534, 10003), (155, 3097, 9051), (163, 10279, 1011),
-    (5949, 162, 13338), (3686, 149, 14130), (163, 3096, 14149), (215, 10039, 940), (2343, 537, 13253),
-    (200, 4414, 12501), (200, 2954, 13107), (242, 9811, 953), (5611, 147, 12749), (118, 20718, 76),
-    (170, 20273, 92), (223, 23140, 77), (319, 19197, 74), (1070, 8540, 65), (441, 20197, 74), (678, 16360, 74),
-    (168, 20370, 576), (193, 24380, 569), (706, 9700, 571), (357, 20186, 654), (3058, 3660, 533),
-    (4075, 2973, 517),
+    (1, 70, 66), (1, 9097, 2089), (1, 5754, 3398), (1, 3951, 8787), (1, 65, 8320), (17, 64, 80),
+    (18, 8471, 3052), (24, 5684, 8484), (17, 71, 15101), (38, 65, 69), (39, 8631, 2514), (33, 5659, 3758),
+    (34, 4091, 9255), (34, 70, 11457), (51, 75, 74), (3958, 65, 2550), (2372, 77, 2556), (1689, 81, 4931),
+    (1173, 75, 8145), (72, 9497, 65), (6569, 87, 4202), (3391, 72, 7144), (3031, 68, 4511), (1783, 65, 15182),
+    (114, 10078, 73), (7297, 65, 6314), (4782, 70, 4879), (3854, 87, 11186), (2162, 66, 12903), (134, 9547, 72),
+    (3625, 365, 5775), (7118, 78, 10075), (4737, 70, 8667), (3215, 72, 12171), (483, 5081, 66),
+    (4176, 307, 11977), (7899, 70, 9850), (6301, 72, 10216), (5919, 582, 64), (5333, 350, 13902),
+    (7339, 75, 12801), (235, 14703, 74), (17, 22440, 6245), (17, 64, 916), (1, 66, 1411), (1, 71, 1927),
+    (55, 20334, 3559), (1426, 75, 1424), (44, 64, 1827), (33, 70, 2955), (5343, 144, 4076), (2890, 69, 2424),
+    (72, 4972, 2275), (1417, 64, 10880), (7684, 136, 2953), (3332, 149, 3462), (2149, 144, 5372),
+    (746, 260, 9712), (131, 10624, 2419), (4780, 147, 3674), (3256, 129, 5229), (132, 2933, 7316),
+    (163, 10646, 2141), (5776, 143, 4765), (2077, 412, 4822), (185, 3178, 10614), (211, 11068, 1768),
+    (3147, 259, 6803), (4369, 136, 10008), (644, 1090, 10071), (235, 20162, 1012), (1422, 1072, 7063),
+    (2680, 276, 9137), (233, 3468, 14580), (170, 20273, 92), (223, 23140, 77), (319, 19197, 74),
+    (340, 24364, 67), (441, 20197, 74), (678, 16360, 74), (269, 23382, 770), (357, 20186, 654),
+    (7849, 1322, 658), (3877, 3111, 719),
 ]
 
 

@@ -19,10 +19,10 @@
 // accumulators, so that a tile's epilogue runs under the next tile's MMAs.
 //
 // What bounds it, and what it reaches on B200 (weights not in L2, calls back to back).  Few tokens: the weight's
-// stream from HBM.  wo (7168 x 16384) 16 tokens 22.5 us (81% of a copy's bandwidth), wq_b (24576 x 1536) 8.6 us,
+// stream from HBM.  wo (7168 x 16384) 16 tokens 21.3 us (85% of a copy's bandwidth), wq_b (24576 x 1536) 8.6 us,
 // [wq_a; wkv_a] (2112 x 7168) 6.6 us, of which a launch with nothing to do is 2.3.  Many tokens: the MMAs; wo 8192
 // tokens 600 us = 3.2e15 operations a second at the clock that 1000 W allow, the tensor pipe active for
-// 87% of the cycles of a full wave.  Small k: the epilogue; 4096 x 32768 x 512 82 us, 3.3 TB/s of y.
+// 87% of the cycles of a full wave.  Small k: the epilogue; 4096 x 32768 x 512 80 us, 3.4 TB/s of y.
 //   An issuing thread alone in its branch took 66 cycles for each MMA and 100 for each TMA load (every operand
 //   moved to a uniform register), 560 a k-step whatever its size, above the MMAs' 512.  With the warp converged
 //   and one elected thread wo 8192 tokens in tiles of 128 went from 1106 to 832 us.
@@ -56,7 +56,7 @@ constexpr int kMaxTok = 256;               // tokens per tile (MMA N)
 constexpr int kMaxSplits = 8;              // CTAs of a portable cluster
 constexpr int kMaxStages = 12;
 // Stages whose weights are requested into L2 before the kernel before has ended.  Four, all, none (us on
-// B200): wo 16 tokens 22.5, 22.3, 23.1; rms_norm_int8 and [wq_a; wkv_a] in a row 8.6, 9.3, 9.1.
+// B200): wo 16 tokens 22.5, 22.3, 23.1 (single CTAs in 2 parts); rms_norm_int8 and [wq_a; wkv_a] in a row 8.6, 9.3, 9.1.
 constexpr int kPrefetch = 4;
 constexpr int kEpiWarps = 8, kEpiThreads = 32 * kEpiWarps;
 constexpr int kStoreWarp = 2 + kEpiWarps;
@@ -152,21 +152,6 @@ __device__ __forceinline__ void put(float v, __half* y) { *y = __float2half_rn(v
 
 // The scale of a token (of the last one for a row past the end, whose products are never written).
 __device__ __forceinline__ float token_scale(const Args& a, int token) { return a.x_scale[min(token, a.m - 1)]; }
-
-// kCols (a power of two) token columns from token0 on for this thread's channel: scaled, rounded and
-// written, by a converged warp.
-template <typename T, int kCols>
-__device__ __forceinline__ void write_columns(const Args& a, const uint32_t (&acc)[kCols], int token0, T* y_channel,
-                                              float w_scale, bool live) {
-  T* y = y_channel + (int64_t)token0 * a.y_stride;
-  const int tokens = live ? a.m - token0 : 0;
-  const float scale = token_scale(a, token0 + (int)(threadIdx.x % kCols));
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    const float v = (float)(int)acc[j] * __shfl_sync(0xffffffffu, scale, j) * w_scale;
-    if (j < tokens) put(v, y + j * a.y_stride);
-  }
-}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -536,8 +521,14 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
       const int row = quarter * 32 + lane, channel = (tn * kGroup + half) * kRows + row, token0 = tt * a.tok;
       const bool live = channel < a.n;
       const float w_scale = live ? a.w_scale[channel] : 0.f;
+      // The scales of the columns that this part adds up (at most 128: thread i has those of i, i + 32, ...).
+      const int first = 4 * split * per, cols = 4 * parts_here;
+      float s_own[kMaxTok / 64];
+#pragma unroll
+      for (int i = 0; i < kMaxTok / 64; ++i) s_own[i] = token_scale(a, token0 + first + 32 * i + lane);
       if (kGroup == 1) cluster_wait();
       if (ok) {
+        const uint32_t per_inv = (65536u + (uint32_t)per - 1) / (uint32_t)per;  // g / per = g per_inv >> 16 for g < 64
         tc_fence_after();
         for (int c = sub * 16; c < a.tok; c += 32) {
           uint32_t r[16];
@@ -546,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
           loaded(r);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int g = c / 4 + j, owner = g / per;
+            const int g = c / 4 + j, owner = (int)(((uint32_t)g * per_inv) >> 16);
             if (owner == split) continue;
             const int part = split < owner ? split : split - 1;
             const uint32_t to = (uint32_t)(owner * kGroup + half);
@@ -559,19 +550,45 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
       __syncwarp();
       cluster_arrive();  // everything sent; completed at the end, before any CTA exits
       if (parts_here > 0 && ok && waiter.wait_warp<true>(bar(kBarParts), 0)) {
-        T* y = static_cast<T*>(a.y) + channel;
+        T* y = static_cast<T*>(a.y) + (int64_t)(token0 + first) * a.y_stride + channel;
         const uint8_t* parts = smem_raw + (staging - raw) + (size_t)row * 16;
-        for (int i = sub; i < parts_here; i += 2) {
-          const int g = split * per + i;
-          uint32_t r[4];
-          tmem_ld4(lanes + (uint32_t)(4 * g), r);
+        const int tokens = min(cols, a.m - token0 - first);
+#pragma unroll
+        for (int i = 0; i < kMaxTok / 64; ++i) {
+          const int c = 32 * i + 16 * sub;  // 16 columns, all of their loads in flight at once
+          if (c >= cols) break;
+          uint32_t r[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + 4 * j < cols) tmem_ld4(lanes + (uint32_t)(first + c + 4 * j), r[j]);
           tc_wait_ld();
-          loaded(r);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) loaded(r[j]);
           for (int p = 0; p < a.splits - 1; ++p) {
-            const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + i) * kRows * 16);
-            r[0] += v.x, r[1] += v.y, r[2] += v.z, r[3] += v.w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (c + 4 * j >= cols) break;
+              const uint4 v = *reinterpret_cast<const uint4*>(parts + (size_t)(p * per + c / 4 + j) * kRows * 16);
+              r[j][0] += v.x, r[j][1] += v.y, r[j][2] += v.z, r[j][3] += v.w;
+            }
           }
-          write_columns<T, 4>(a, r, token0 + 4 * g, y, w_scale, live);
+          // All values first, then the stores: a store under a condition between two shuffles costs 100 cycles.
+          T v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            put((float)(int)r[j / 4][j % 4] * __shfl_sync(0xffffffffu, s_own[i], 16 * sub + j) * w_scale, v + j);
+          if (live) {
+            T* yc = y + c * a.y_stride;
+            if (c + 16 <= tokens) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) yc[j * a.y_stride] = v[j];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (c + j < tokens) yc[j * a.y_stride] = v[j];
+            }
+          }
+          __syncwarp();
         }
       }
     }
@@ -730,28 +747,30 @@ constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
 // Estimated microseconds of a call, up to a constant.  The tiles run in waves; a k-step of a tile takes the
 // longer of its MMAs and the fill of a CTA's shared memory, an unsplit tile at least the epilogue of the tile
-// before it.  HBM's time for the operands and y overlaps in part.  The constants are fitted to 2,300
+// before it.  HBM's time for the operands and y overlaps in part.  The constants are fitted to 3,000
 // calls measured on B200 (1 to 8000 tokens, twelve n x k from 300 x 300 to 512 x 16384 and 24576 x 1536, every
-// variant, bf16 out): the variant with the least estimate is on average 1.8% slower than the fastest
-// measured, 17% at worst.
+// variant, bf16 out): the variant with the least estimate is on average 1.4% slower than the fastest
+// measured, 15% at worst.
 double estimate(int m, int n, int k, int size, int group, int tok, int splits, int sms) {
   const double k_steps = (k + kBoxK - 1) / kBoxK, tiles = (double)((n + kRows * group - 1) / (kRows * group)) *
                                                           ((m + tok - 1) / tok);
   const double slots = kClusters[group * splits] * (sms / 148.0);
-  const double step = fmax(fmax(0.986 * tok, 7.773 * (16 + tok / 8.0 / group)), 60.6) * 1e-3;
-  const double epilogue = (4.286 * tok + 418.) * 1e-3, steps = ceil(k_steps / splits) * step;
+  const double step = fmax(fmax(0.968 * tok, 7.719 * (16 + tok / 8.0 / group)), 101.6) * 1e-3;
+  const double epilogue = (3.358 * tok + 472.) * 1e-3, steps = ceil(k_steps / splits) * step;
   const double tiles_us = ceil(tiles / slots) * (splits == 1 ? fmax(steps, epilogue) : steps);
-  const double hbm_us = ((double)n * k + (double)m * k + 1.764 * size * m * n) / 9.67e6;
-  return (group == 2 ? 0.589 : 0.) + fmax(tiles_us, hbm_us) + 0.723 * fmin(tiles_us, hbm_us) +
-         (splits == 1 ? epilogue : 0.366 + 0.035 * tok);
+  const double hbm_us = ((double)n * k + (double)m * k + 2.04 * size * m * n) / 10.98e6;
+  const double last = splits == 1 ? epilogue + (group == 2 ? 1.445 : 0.)
+                                  : 0.614 + 0.0189 * tok + 0.273 * splits - (group == 2 ? 0.507 : 0.);
+  return fmax(tiles_us, hbm_us) + 0.705 * fmin(tiles_us, hbm_us) + last;
 }
 
 // The variant with the least estimate.  Examples (us measured, the chosen one first):
-//   wo (7168 x 16384), 16 tokens: 2 parts 23.1, unsplit 25.1;  64 tokens: pairs in 2 parts 24.6, single
-//   CTAs in 2 parts 25.6, pairs unsplit 27.8;  256 tokens: pairs of 128 33.7, single CTAs of 128 37.3, pairs of
-//   256 in 2 parts 36.9;  [wq_a; wkv_a] (2112 x 7168), 16 tokens: 6 parts 6.6, unsplit 10.3;
-//   wq_b (24576 x 1536), 4096 tokens: pairs of 256 109, single CTAs 131;
-//   20000 x 128, 4096 tokens: single CTAs 48, pairs 57.
+//   wo (7168 x 16384), 16 tokens: pairs in 2 parts 21.3, single CTAs in 2 parts 22.5, unsplit 25.1;
+//   64 tokens: pairs in 2 parts 21.8, single CTAs in 2 parts 24.1, unsplit 26.6;  256 tokens: pairs of 256 in 2
+//   parts 30.4, pairs of 128 33.4, single CTAs of 128 37.3;
+//   [wq_a; wkv_a] (2112 x 7168), 16 tokens: pairs in 4 parts 6.6, single CTAs in 6 parts 6.7, unsplit 10.3;
+//   wq_b (24576 x 1536), 4096 tokens: pairs of 256 105, single CTAs 130;
+//   20000 x 128, 4096 tokens: single CTAs 45, pairs 54.
 Plan make_plan(int m, int n, int k, int size, int sms) {
   constexpr int kTokens[] = {64, 96, 128, 160, 192, 224, 256}, kSplits[] = {1, 2, 3, 4, 6};
   Plan best{};
