@@ -244,6 +244,12 @@ VARIANT_SHAPES = [
     (2680, 276, 9137), (233, 3468, 14580), (170, 20273, 92), (223, 23140, 77), (319, 19197, 74),
     (340, 24364, 67), (441, 20197, 74), (678, 16360, 74), (269, 23382, 770), (357, 20186, 654),
     (7849, 1322, 658), (3877, 3111, 719),
+    (7, 8465, 7363), (1, 5743, 11131), (22, 8773, 8607), (18, 66, 16005), (47, 8535, 10130), (45, 5640, 12628),
+    (1446, 69, 5406), (972, 66, 8517), (2082, 274, 5875), (2862, 73, 16210), (4345, 75, 11772),
+    (3708, 70, 16189), (474, 2943, 10323), (5853, 65, 16150), (4674, 119, 16191), (514, 3015, 14526),
+    (5480, 124, 16720), (421, 4734, 16695), (22, 20313, 11209), (524, 808, 4976), (707, 340, 9612),
+    (1092, 857, 5245), (797, 823, 4691), (709, 546, 10453), (531, 1649, 5748), (908, 516, 11792),
+    (1310, 1259, 7589), (1117, 780, 9094), (1464, 1172, 9467), (1021, 1069, 9215),
 ]
 
 

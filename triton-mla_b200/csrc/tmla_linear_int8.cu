@@ -747,21 +747,21 @@ constexpr int kClusters[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 
 // Estimated microseconds of a call, up to a constant.  The tiles run in waves; a k-step of a tile takes the
 // longer of its MMAs and the fill of a CTA's shared memory, an unsplit tile at least the epilogue of the tile
-// before it.  HBM's time for the operands and y overlaps in part.  The constants are fitted to 3,000
-// calls measured on B200 (1 to 8000 tokens, twelve n x k from 300 x 300 to 512 x 16384 and 24576 x 1536, every
-// variant, bf16 out): the variant with the least estimate is on average 1.4% slower than the fastest
-// measured, 15% at worst.
+// before it.  HBM's time for the operands and y overlaps in part; further token tiles read the weight again, from
+// L2.  The constants are fitted to 5,700 calls measured on B200 (1 to 8000 tokens, n x k from 300 x 300 to
+// 512 x 16384 and 24576 x 1536, every variant, bf16 out): the variant with the least estimate is on average
+// 1.3% slower than the fastest measured, 7% or less in 95% of the sizes, 18% at worst.
 double estimate(int m, int n, int k, int size, int group, int tok, int splits, int sms) {
-  const double k_steps = (k + kBoxK - 1) / kBoxK, tiles = (double)((n + kRows * group - 1) / (kRows * group)) *
-                                                          ((m + tok - 1) / tok);
+  const double k_steps = (k + kBoxK - 1) / kBoxK, n_tiles = (n + kRows * group - 1) / (kRows * group),
+               t_tiles = (m + tok - 1) / tok;
   const double slots = kClusters[group * splits] * (sms / 148.0);
-  const double step = fmax(fmax(0.968 * tok, 7.719 * (16 + tok / 8.0 / group)), 101.6) * 1e-3;
-  const double epilogue = (3.358 * tok + 472.) * 1e-3, steps = ceil(k_steps / splits) * step;
-  const double tiles_us = ceil(tiles / slots) * (splits == 1 ? fmax(steps, epilogue) : steps);
-  const double hbm_us = ((double)n * k + (double)m * k + 2.04 * size * m * n) / 10.98e6;
-  const double last = splits == 1 ? epilogue + (group == 2 ? 1.445 : 0.)
-                                  : 0.614 + 0.0189 * tok + 0.273 * splits - (group == 2 ? 0.507 : 0.);
-  return fmax(tiles_us, hbm_us) + 0.705 * fmin(tiles_us, hbm_us) + last;
+  const double step = fmax(0.85 * tok, 6.8 * (16 + tok / 8.0 / group)) * 1e-3;
+  const double epilogue = (4.06 * tok + 519.) * 1e-3, steps = ceil(k_steps / splits) * step;
+  const double tiles_us = ceil(n_tiles * t_tiles / slots) * (splits == 1 ? fmax(steps, epilogue) : steps);
+  const double hbm_us = ((double)n * k * (1 + 0.28 * (t_tiles - 1)) + (double)m * k + 0.34 * size * m * n) / 5.38e6;
+  const double last = splits == 1 ? epilogue + (group == 2 ? 0.64 : 0.)
+                                  : 0.985 + 0.0247 * tok + 0.082 * splits - (group == 2 ? 0.805 : 0.);
+  return fmax(tiles_us, hbm_us) + 0.28 * fmin(tiles_us, hbm_us) + last;
 }
 
 // The variant with the least estimate.  Examples (us measured, the chosen one first):
@@ -770,7 +770,8 @@ double estimate(int m, int n, int k, int size, int group, int tok, int splits, i
 //   parts 30.4, pairs of 128 33.4, single CTAs of 128 37.3;
 //   [wq_a; wkv_a] (2112 x 7168), 16 tokens: pairs in 4 parts 6.6, single CTAs in 6 parts 6.7, unsplit 10.3;
 //   wq_b (24576 x 1536), 4096 tokens: pairs of 256 105, single CTAs 130;
-//   20000 x 128, 4096 tokens: single CTAs 45, pairs 54.
+//   20000 x 128, 4096 tokens: single CTAs 45, pairs 54;  32768 x 512, 4096 tokens: single CTAs 81, pairs 92;
+//   4001 x 2001, 77 tokens: single CTAs of 64 tokens 5.9, pairs of 96 in 2 parts 6.3, pairs of 64 in 2 parts 7.0.
 Plan make_plan(int m, int n, int k, int size, int sms) {
   constexpr int kTokens[] = {64, 96, 128, 160, 192, 224, 256}, kSplits[] = {1, 2, 3, 4, 6};
   Plan best{};
