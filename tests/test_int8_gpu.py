@@ -168,6 +168,19 @@ def test_special_rows(device, dtype, k):
     assert torch.equal(torch.isnan(y[:, 0]).cpu(), torch.tensor([False, True, True, True, False, False, False]))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("k", [100, 1001, 7168])
+def test_squares_beyond_fp32_make_the_norm_zero(device, dtype, k):
+    """The sum of squares is infinite, so 1 / rms is 0; the other rows are as they were."""
+    g = _gen(device, k)
+    x = torch.randn(3, k, generator=g, device=device).to(dtype)
+    x[1] = 1e20
+    q, scale, _ = layer_ops.rms_norm_int8(x, torch.ones(k, dtype=dtype, device=device))
+    assert not bool(q[1].any()) and float(scale[1]) == 2.0 ** -126
+    want_q, want_scale, _ = layer_ops.rms_norm_int8(x[::2].contiguous(), torch.ones(k, dtype=dtype, device=device))
+    assert torch.equal(q[::2], want_q) and torch.equal(scale[::2], want_scale)
+
+
 def test_empty_batches(device):
     x = torch.zeros(0, 64, device=device, dtype=torch.bfloat16)
     q, s = layer_ops.quantize_int8(x)

@@ -320,8 +320,9 @@ __global__ void __launch_bounds__(kMaxThreads) values_kernel(const Args a) {
   }
 }
 
-// Rows too long for the registers of a block, by vectors or value by value: the row is read a second time (from L1 / L2) for its integers.  With a residual the
-// second pass reads h, which the same thread has written.
+// Rows too long for the registers of a block, by vectors or value by value: the row is read a second
+// time (from L1 / L2) for its integers.  With a residual the second pass reads h, which the same thread
+// has written.
 template <typename T, bool kNorm, bool kAligned>
 __global__ void __launch_bounds__(kMaxThreads) loop_kernel(const Args a) {
   __shared__ uint32_t s_mx[1][32];
