@@ -373,8 +373,10 @@ int64_t tmla_linear_workspace_bytes(int32_t m, int32_t n, int32_t k, int32_t gro
    tmla_quantize_int8 -> tmla_linear_int8 (wo) around the decode. */
 
 /* int8 rows with a scale each.  dtype (TMLA_DTYPE_*) is the type of x, residual, weight and h.
-   tmla_quantize_int8: scale[i] = max(max_j |x[i, j]| / 127, 2^-126), q[i, j] = x[i, j] / scale[i]
-   rounded to nearest (ties to even); weight and residual must be NULL.  Also for a weight
+   tmla_quantize_int8: scale[i] = max(max_j |x[i, j]| / 127, 2^-126), q[i, j] = x[i, j] * (1 / scale[i])
+   rounded to nearest (ties to even), where the quotient, its reciprocal and the product are each
+   rounded to fp32: within half a step and 2^-16 of x[i, j] / scale[i], so a quotient next to half an
+   integer may go to either neighbour.  weight and residual must be NULL.  Also for a weight
    [n, k], whose rows are output channels.
    tmla_rms_norm_int8: h = x + residual rounded to dtype (h = x without a residual; h is written
    only with one), y = h * weight / sqrt(mean(h^2) + eps) in fp32, and y quantised as above.  h may

@@ -267,7 +267,8 @@ def quantize_int8(x: torch.Tensor, overlap: bool = False):
     """int8 rows of ``x`` [m, k] with one scale each: ``(q, scale)`` with q int8 [m, k], scale
     fp32 [m] and ``x ~ q * scale[:, None]`` (C ABI: ``tmla_quantize_int8``).
 
-    scale = max(max |row| / 127, 2^-126); q = row / scale rounded to nearest.  For activations
+    scale = max(max |row| / 127, 2^-126); q = row * (1 / scale) rounded to nearest (ties to even), each
+    operation in fp32, so q is within half a step and 2^-16 of row / scale.  For activations
     (a scale per token) and for weights [n, k] (a scale per output channel).  A row with a NaN
     or an infinity gets scale NaN and zeros.  Rows of q start on 16-byte boundaries, so q's row
     stride is k rounded up to 16 (the padding bytes are not written).  Bf16, fp16 or fp32, any
