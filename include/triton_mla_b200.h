@@ -240,7 +240,9 @@ size_t tmla_params_bytes(void);
 /* Layer-op flag: launch as a programmatic dependent of the preceding kernel in the stream
    (its launch and the op's weight-tile loads overlap that kernel's end; every input other
    than the weights is read only after that kernel has completed).  Do not set it when the
-   preceding kernel writes w_kv_b / norm_weight. */
+   preceding kernel writes w_kv_b / norm_weight.  Kernels before the preceding one may write them:
+   every kernel of this library lets its successor be scheduled only after its own wait for its
+   predecessor. */
 #define TMLA_LAYER_FLAG_PDL 1
 
 typedef struct TmlaQPrepParams {

@@ -547,6 +547,27 @@ def test_a_weight_written_just_before(device):
         _compare_linear(y, x, s, wq, ws)
 
 
+@pytest.mark.parametrize("m,n,k", [(16, 2112, 7168), (256, 2048, 4096), (600, 4096, 1024)])
+def test_a_weight_written_two_kernels_before(device, m, n, k):
+    """With ``overlap`` only the kernel just before may not write the weight: one product (with another weight) lies
+    between the quantisation of the weight and its product, which loads it ahead of its wait."""
+    g = _gen(device, 35)
+    x1, s1 = _int8(m, k, g, device), torch.rand(m, generator=g, device=device)
+    w1, v1 = _int8(n, k, g, device), torch.rand(n, generator=g, device=device)
+    x2, s2 = _int8(16, 1536, g, device), torch.rand(16, generator=g, device=device)
+    for i in range(20):
+        w = torch.randn(24576, 1536, generator=g, device=device).to(torch.bfloat16)
+        torch.cuda.synchronize()
+        w2, v2 = layer_ops.quantize_int8(w)
+        y1 = layer_ops.linear_int8(x1, s1, w1, v1)
+        y2 = layer_ops.linear_int8(x2, s2, w2, v2, overlap=True)
+        torch.cuda.synchronize()
+        assert torch.equal(y2, layer_ops.linear_int8(x2, s2, w2, v2))
+        if i == 0:
+            _compare_linear(y1, x1, s1, w1, v1)
+            _compare_linear(y2, x2, s2, w2, v2)
+
+
 def test_no_gradient_passes(device):
     x = torch.randn(4, 64, device=device, requires_grad=True)
     w = torch.ones(64, device=device, requires_grad=True)

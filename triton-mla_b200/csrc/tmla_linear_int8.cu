@@ -338,6 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
     // Into L2 the weights may come at any time (a write by the kernel before would update them there).
     for (int s = early; s < pre && s < kPrefetch; ++s) tma_prefetch_2d(&tm_w, (ks0 + s) * kBoxK, w_row, elected);
     griddep_wait();
+    // Only now may the next kernel be scheduled: its loads ahead of its own wait count on every kernel before this one
+    // having completed.  A single CTA holds its TMEM first, so that the next one cannot keep it out.
+    if (kGroup == 2) griddep_launch_dependents();
     for (int s = 0; s < pre; ++s) {
       if (s >= early && (!stalled || s > 0)) load_w(s, ks0 + s, w_row);
       if (!stalled || s > 0) load_x(s, ks0 + s, x_row);
@@ -373,10 +376,11 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
   const Waiter waiter{abort_flag, a.status, a.wait_ns};
 
   if (warp == 0) {
-    // Past this the next kernel may be scheduled; this CTA holds its TMEM already, so it cannot be kept out.
-    griddep_launch_dependents();
     // The whole warp runs this (its operands stay warp-uniform); one thread issues.
-    if (kGroup == 2) first_round();
+    if (kGroup == 1)
+      griddep_launch_dependents();  // first_round has waited
+    else
+      first_round();
     int s = pre == a.stages ? 0 : pre;               // ring position, and how often the ring has wrapped
     uint32_t round = pre == a.stages ? 1 : 0;
     bool ok = true;
