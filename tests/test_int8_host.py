@@ -115,3 +115,21 @@ def test_int8_operators_have_meta_kernels():
     wq = torch.empty(70, 1001, dtype=torch.int8, device="meta")
     y = ops.linear_int8(q, scale, wq, torch.empty(70, device="meta"), torch.float16, False, None)
     assert y.shape == (5, 70) and y.dtype == torch.float16 and y.stride() == (72, 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("m,n", [(1, 1), (32, 249), (5, 1001), (3, 64), (0, 7), (4, 0)])
+def test_padded_rows_lie_in_their_own_storage(dtype, m, n):
+    """Rows of y, h and q are padded to 16 bytes, the last one too: what a TMA store may write there is the tensor's."""
+    ops = torch.ops.triton_mla
+    wq = torch.empty(n, 64, dtype=torch.int8, device="meta")
+    xq, xs = torch.empty(m, 64, dtype=torch.int8, device="meta"), torch.empty(m, device="meta")
+    tensors = [ops.linear_int8(xq, xs, wq, torch.empty(n, device="meta"), dtype, False, None)]
+    if n:
+        x, w = torch.empty(m, n, dtype=dtype, device="meta"), torch.empty(n, dtype=dtype, device="meta")
+        q, _, h = ops.rms_norm_int8(x, w, 1e-6, x, None, False)
+        tensors += [q, h, ops.quantize_int8(x, False)[0]]
+    for t in tensors:
+        row = -(-n * t.element_size() // 16) * 16
+        assert t.shape == (m, n) and t.stride(1) == 1 and (m < 2 or t.stride(0) * t.element_size() == max(row, t.element_size()))
+        assert t.untyped_storage().nbytes() >= m * row and t.storage_offset() == 0 and not t._is_view()

@@ -108,10 +108,14 @@ void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& le
 // boundaries (a row stride of k or n rounded up), as the kernels' vector accesses and TMA want them.  Outputs come
 // from the caching allocator, the launches go on the current stream of the inputs' device.
 
-// An [m, n] tensor whose rows start on 16-byte boundaries.
+// An [m, n] tensor whose rows start on 16-byte boundaries.  Its storage holds the last row's padding too, which the
+// product's TMA stores fill (an [m, n] tensor of these strides alone would end with the last row's values).
 at::Tensor aligned_rows(int64_t m, int64_t n, const at::TensorOptions& options, at::ScalarType dtype) {
   const int64_t per = 16 / (int64_t)at::elementSize(dtype);
-  return at::empty_strided({m, n}, {std::max<int64_t>(1, (n + per - 1) / per * per), 1}, options.dtype(dtype));
+  const int64_t stride = std::max<int64_t>(1, (n + per - 1) / per * per);
+  at::Tensor t = at::empty({m, stride}, options.dtype(dtype));
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(c10::IntArrayRef{m, n}, c10::IntArrayRef{stride, 1});
+  return t;
 }
 at::Tensor int8_rows(const at::Tensor& x) { return aligned_rows(x.size(0), x.size(1), x.options(), at::kChar); }
 
