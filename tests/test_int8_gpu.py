@@ -623,3 +623,31 @@ def test_a_timed_out_wait_returns_cleanly(device, m, n, k):
     torch.cuda.synchronize()
     assert read_status(device) == 0
     _compare_linear(y, xq, xs, wq, ws)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 7211), (10, 2488, 1186), (1, 64, 1150), (16, 2112, 7168), (130, 1000, 4000)])
+def test_timed_out_parts_of_a_split_tile(device, m, n, k):
+    """A cluster whose first CTA gives up: the parts that the others send to it, and it to them, are late or never
+    come.  The next call, launched right behind, runs on the same SMs and is exact, time after time."""
+    import ctypes
+
+    from triton_mla import _lib
+    from triton_mla.kernel import _status_word
+
+    g = _gen(device, 12)
+    xq, wq = _int8(m, k, g, device), _int8(n, k, g, device)
+    xs, ws = torch.rand(m, generator=g, device=device), torch.rand(n, generator=g, device=device)
+    y, y2 = torch.empty(m, n, device=device), torch.empty(m, n, device=device)
+    args = [xq.data_ptr(), xq.stride(0), xs.data_ptr(), wq.data_ptr(), wq.stride(0), ws.data_ptr()]
+    stalled = _lib.TmlaLinearInt8Params(*args, y.data_ptr(), n, m, n, k, _lib.DTYPE_FP32, _lib.LINEAR_FLAG_TEST_STALL,
+                                        _status_word(device).data_ptr(), 300_000)
+    whole = _lib.TmlaLinearInt8Params(*args, y2.data_ptr(), n, m, n, k, _lib.DTYPE_FP32, 0, None, 0)
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    read_status(device)
+    for _ in range(20):
+        y2.zero_()
+        assert _lib.load().tmla_linear_int8(ctypes.byref(stalled), stream) == 0
+        assert _lib.load().tmla_linear_int8(ctypes.byref(whole), stream) == 0
+        torch.cuda.synchronize()
+        assert read_status(device) == _lib.STATUS_TIMEOUT
+        _compare_linear(y2, xq, xs, wq, ws)

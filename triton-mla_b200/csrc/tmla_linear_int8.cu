@@ -31,7 +31,7 @@
 //
 // Every wait is bounded (2 s by default): on expiry the kernel sets TMLA_STATUS_TIMEOUT, stops,
 // drains the copies and MMAs that it issued, leaves the tiles that it could not finish unwritten,
-// frees TMEM and returns.
+// waits for what others are still sending it, frees TMEM and returns.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -73,6 +73,7 @@ constexpr int kBoxChannels = sizeof(T) == 2 ? 64 : kRows;
 constexpr int kMaxRows = 1 << 30;          // tokens and channels: row numbers past a tile's end stay in int
 constexpr uint32_t kSmemMax = 227 * 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint64_t kInFlightNs = 100000ull;  // how long a CTA that gave up keeps its memory, far above a transfer's latency
 
 // After the ring and the staged chunks: barriers full / empty per stage, accumulator full / empty (two),
 // "MMAs done", chunk full / empty, the parts of a split tile; the TMEM address, the abort flag.
@@ -649,6 +650,15 @@ __global__ void __launch_bounds__(kThreads, 1) int8_kernel(const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
+    // A CTA that gave up has not waited for all that is on its way to it: the parts of a split tile (the cluster barrier
+    // orders their sending, not their landing), a pair's arrivals, copies past a short limit.  It keeps its shared memory
+    // and TMEM for as long as they can take: a CTA that exits under a landing transfer loses the context.
+    if (*abort_flag) {
+      const uint64_t t0 = globaltimer();
+      while (globaltimer() - t0 < kInFlightNs) {
+      }
+      __syncwarp();
+    }
     tc_fence_after();
     tmem_dealloc_g<kGroup>(tmem, (uint32_t)a.tmem_cols);
   }
