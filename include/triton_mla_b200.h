@@ -383,7 +383,8 @@ int64_t tmla_linear_workspace_bytes(int32_t m, int32_t n, int32_t k, int32_t gro
    tmla_rms_norm_int8: h = x + residual rounded to dtype (h = x without a residual; h is written
    only with one), y = h * weight / sqrt(mean(h^2) + eps) in fp32, and y quantised as above.  h may
    be x or residual themselves (same strides), not another overlap of them.
-   A row that holds a NaN or an infinity gets scale NaN and integers 0.  |q| <= 127 always.
+   A row that holds a NaN or an infinity (or whose y does, in fp32) gets scale NaN and integers 0.  Squares that
+   sum past fp32 make y 0; products h * weight past fp32 do no harm (y is formed in another order).  |q| <= 127 always.
    Any m (below 2^31), k (1 to 2^30) and row strides >= k; rows that start on 16-byte boundaries (8 for q from a
    16-bit x) are moved in whole vectors.  Bytes of q past k in a row are not written. */
 typedef struct TmlaInt8RowsParams {

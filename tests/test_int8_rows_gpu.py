@@ -1,5 +1,5 @@
 """int8 rows (``layer_ops.quantize_int8``, ``rms_norm_int8``) at the borders of their definition: the integers bit for
-bit, rows of every kernel variant.
+bit, rows of every kernel variant, products that pass fp32.
 
 Tolerances of a norm, in units u = 2^-24 as in ``test_int8_gpu``, for every variant: a thread adds up to 64 squares
 in a row (8 vectors of 8 values, or k / 1024 + 8 for looped rows) and 10 more across threads.  rstd is off by half of
@@ -117,6 +117,42 @@ def test_integers_at_the_ends_of_fp32(device):
         assert torch.equal(scale, _by_127(x.abs().amax(-1)).clamp_min(TINY))
         assert torch.equal(q, _integers(x, scale))
         assert int(q[0].abs().max()) == 127 and not bool(q[3].any())
+
+
+# ----------------------------------------------------------------------------- products and squares past fp32
+FAR_LAYOUTS = [(100, 104, 0), (7168, 7168, 0), (32768, 32768, 0), (1001, 1003, 1), (10001, 10003, 1), (40000, 40000, 0)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("k,stride,offset", FAR_LAYOUTS)
+def test_products_beyond_fp32(device, dtype, k, stride, offset):
+    """|h w| above 3.4e38 with finite h and w is not a row without a scale: where the squares sum past fp32 too the
+    norm is 0, where they do not y is what its formula says.  An infinity itself still leaves no scale."""
+    g = _gen(device, k)
+    x = _rows(7, k, stride, offset, dtype, g, device)
+    ordinary = x.clone()
+    w = (1 + 0.2 * torch.randn(k, generator=g, device=device)).to(dtype)
+    w[1], w[2] = 4.0, 1e30
+    x[1, 1] = 2e38                                        # h w = 8e38 and h^2 past fp32: zeros
+    x[2, 2] = 1e12                                        # h w = 1e42, h^2 = 1e24: an ordinary norm
+    x[3] = 1e15
+    x[4, 1] = float("inf")
+    x[5, 0] = float("nan")
+    x[5, 2] = 1e12
+    x[6, 1], x[6, 2] = 2e38, float("inf")
+    for residual in (None, torch.zeros_like(x)):
+        q, s, _ = layer_ops.rms_norm_int8(x, w, residual=residual)
+        assert float(s[1]) == TINY and not bool(q[1].any())
+        for bad in (4, 5, 6):
+            assert bool(torch.isnan(s[bad])) and not bool(q[bad].any())
+        for row in (0, 2, 3):
+            _check_norm(x[row:row + 1], w, residual=None if residual is None else residual[row:row + 1])
+            f = x[row].double()
+            y = f * w.double() / (f.square().mean() + 1e-6).sqrt()
+            assert abs(float(s[row]) - float(y.abs().max() / 127)) <= 1e-5 * float(s[row])
+    w[2] = float("inf")
+    q, s, _ = layer_ops.rms_norm_int8(ordinary, w)
+    assert bool(torch.isnan(s).all()) and not bool(q.any()), "a weight without a value leaves no row a scale"
 
 
 def test_eps_of_zero(device):

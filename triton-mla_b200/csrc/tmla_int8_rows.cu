@@ -11,11 +11,11 @@
 // norm is of the residual stream as stored), the int8 values are rounded once, to nearest even.
 //
 // Bound: HBM bandwidth.  Measured on B200 (inputs beyond L2, back to back): quantise 8192 x 7168 bf16
-// 28.4 us (6.2 TB/s, 95% of a copy), norm with residual 69.9 us (5.9 TB/s, 90%), norm without
-// 40.5 us; one token 2.0-2.7 us, which is launch and one trip to memory.
+// 28.3 us (6.2 TB/s, 95% of a copy), norm with residual 70 us (5.9 TB/s, 90%), norm without
+// 41.7 us; one token 2.0-2.7 us, which is launch and one trip to memory.
 //
 // A row that holds a NaN or an infinity has no scale: its scale is NaN and its integers are 0,
-// so every product with it is NaN.  The maximum keeps a NaN.
+// so every product with it is NaN.  The maximum keeps a NaN.  Products h w beyond fp32 alone are not that (far_row).
 #include "tmla_common.cuh"
 #include "tmla_ptx.cuh"
 
@@ -174,6 +174,31 @@ __device__ __forceinline__ void row_scale(float mx, float sum, int k, float eps,
   inv = 1.f / scale;
 }
 
+// A row whose largest |h w| is infinite.  That is a row without a scale if h or w holds an infinity, but finite h and w
+// may only have a product past fp32: y is then formed as (h rstd) w, which is finite unless y itself is not (and 0 where
+// the squares sum past fp32 too, rstd being 0).  Rare, so value by value: each warp looks for the maximum over the whole
+// row, without a barrier (rows of a block may differ), then every thread writes its values.  h is the row as stored.
+template <typename T>
+__device__ __forceinline__ void far_row(const T* h, const T* w, int8_t* q, float* scale_out, int k, float sum,
+                                        float eps) {
+  __syncwarp();  // h may have been written by this row's other threads (of other warps: a barrier came since)
+  const float rstd = rsqrtf(sum / (float)k + eps);
+  float top = 0.f;
+  for (int j = threadIdx.x & 31; j < k; j += 32) top = max_nan(top, fabsf(to_float(h[j]) * rstd * to_float(w[j])));
+  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+  float scale, one, inv;
+  row_scale<false>(top, 0.f, k, eps, scale, one, inv);
+  if (threadIdx.x == 0) *scale_out = scale;
+  for (int j = threadIdx.x; j < k; j += blockDim.x)
+    q[j] = (int8_t)round_bits(inv == 0.f ? 0.f : to_float(h[j]) * rstd * to_float(w[j]), inv);
+}
+
+// For rows_kernel as a call: within it the kernel of 4 vectors a thread takes 42.2 us for 8192 x 7168 instead of 41.6.
+template <typename T>
+__device__ __noinline__ void far_row_call(const T* h, const T* w, int8_t* q, float* scale, int k, float sum, float eps) {
+  far_row(h, w, q, scale, k, sum, eps);
+}
+
 // The row's running maximum of |y| (up to rstd) and sum of squares over one value.
 template <bool kNorm>
 __device__ __forceinline__ float visit(float h, float w, float& mx, float& sum) {
@@ -189,9 +214,11 @@ __device__ __forceinline__ float visit(float h, float w, float& mx, float& sum) 
 // to kVecs vectors of its row, vector i of thread t being number i * threads + t, and the first
 // k % N threads one value each of the row's end.  Loads are predicated, not branched around, so
 // that all of a thread's are in flight at once.  The row stays packed in T across the reduction (4
-// registers per vector); h w is formed again after it.
+// registers per vector); h w is formed again after it.  One or two vectors a thread are rows of 64 threads at most, in
+// blocks of 128, of which an SM's registers are to hold 12 and 9 (65536 x 256, norm with residual: 22.4 us, else 24.6).
 template <typename T, int kVecs, bool kNorm>
-__global__ void __launch_bounds__(kVecs >= 4 ? 512 : kMaxThreads, kVecs == 4 ? 2 : 1) rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kVecs >= 4 ? 512 : 128, kVecs >= 8 ? 1 : kVecs == 4 ? 2 : kVecs == 2 ? 9 : 12)
+    rows_kernel(const Args a) {
   __shared__ uint32_t s_mx[32][32];
   __shared__ float s_sum[kNorm ? 32 : 1][32];
   constexpr int N = kPer<T>;
@@ -253,6 +280,11 @@ __global__ void __launch_bounds__(kVecs >= 4 ? 512 : kMaxThreads, kVecs == 4 ? 2
   h_last = visit<kNorm>(h_last, w_last, mx, sum);
   reduce_row<kNorm>(mx, sum, s_mx, s_sum);
   if (row >= a.m) return;
+  if (kNorm && mx == INFINITY) {
+    far_row_call(a.r != nullptr ? static_cast<const T*>(a.h) + row * a.h_stride : x, static_cast<const T*>(a.w),
+                 a.q + row * a.q_stride, a.scale + row, a.k, sum, a.eps);
+    return;
+  }
   float scale, rstd, inv;
   row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
   if (t == 0) a.scale[row] = scale;
@@ -313,6 +345,11 @@ __global__ void __launch_bounds__(kMaxThreads) values_kernel(const Args a) {
   for (int i = 0; i < kValues; ++i) h[i] = visit<kNorm>(h[i], wv[i], mx, sum);
   reduce_row<kNorm>(mx, sum, s_mx, s_sum);
   if (row >= a.m) return;
+  if (kNorm && mx == INFINITY) {
+    far_row(a.r != nullptr ? static_cast<const T*>(a.h) + row * a.h_stride : x, static_cast<const T*>(a.w),
+            a.q + row * a.q_stride, a.scale + row, a.k, sum, a.eps);
+    return;
+  }
   float scale, rstd, inv;
   row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
   if (t == 0) a.scale[row] = scale;
@@ -366,6 +403,10 @@ __global__ void __launch_bounds__(kMaxThreads) loop_kernel(const Args a) {
     visit<kNorm>(to_float(v), kNorm ? to_float(w[j]) : 1.f, mx, sum);
   }
   reduce_row<kNorm>(mx, sum, s_mx, s_sum);
+  if (kNorm && mx == INFINITY) {
+    far_row(res ? h : x, w, a.q + row * a.q_stride, a.scale + row, a.k, sum, a.eps);
+    return;
+  }
   float scale, rstd, inv;
   row_scale<kNorm>(mx, sum, a.k, a.eps, scale, rstd, inv);
   if (threadIdx.x == 0) a.scale[row] = scale;
@@ -414,7 +455,7 @@ template <typename T, bool kNorm>
 cudaError_t run(const Args& a, bool aligned, cudaStream_t stream) {
   const int vecs = a.k / kPer<T> > 0 ? a.k / kPer<T> : 1;
   if (!aligned && a.k <= kValues * kMaxThreads) {
-    // 333 x 1003 fp32 (norm with residual): 3.6 us, against 6.6 with the loop kernel below.
+    // 333 x 1003 fp32 (norm with residual): 2.6 us, against 6.6 with the loop kernel below.
     const int threads = (a.k + 32 * kValues - 1) / (32 * kValues) * 32, rows = threads >= 128 ? 1 : 128 / threads;
     return launch(values_kernel<T, kNorm>, dim3((unsigned)((a.m + rows - 1) / rows)), dim3(threads, rows), a, stream);
   }

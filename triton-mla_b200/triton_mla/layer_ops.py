@@ -291,7 +291,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     the new residual: a new tensor (rows on 16-byte boundaries, as q's), or ``residual_out``, which may be
     ``residual`` or ``x`` itself (but overlap them in no other way).  Without a residual h is None
     and x is normalised as it is.  Squares that sum past fp32 (|h| above 1.8e19) make the norm 0,
-    as any fp32 norm does: zeros with the smallest scale.
+    as any fp32 norm does: zeros with the smallest scale.  A NaN or an infinity in h or weight leaves a row without
+    a scale (NaN, and zeros); a product h * weight past fp32 alone does not.
 
     The int8 operators always launch as programmatic dependents (they wait for the preceding
     kernel before they touch memory); ``overlap`` also lets the weight loads run before that
