@@ -223,6 +223,10 @@ const char* tmla_error_string(int code);
 const char* tmla_last_cuda_error(void);
 int tmla_abi_version(void);
 
+/* A status word that the library owns on the current device (4 bytes, zero when the library is loaded, kept until the
+   process exits), for callers without one of their own.  May be called during a stream capture. */
+int tmla_status_word(int32_t** word);
+
 /* sizeof(TmlaDecodeParams) as compiled, so an FFI binding can check its mirror of the struct. */
 size_t tmla_params_bytes(void);
 

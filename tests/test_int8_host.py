@@ -90,6 +90,10 @@ def test_null_parameter_structs_are_refused():
         assert fn(None, None) == _lib.ERR_INVALID_ARG
 
 
+def test_the_status_word_needs_somewhere_to_go():
+    assert _lib.load().tmla_status_word(None) == _lib.ERR_INVALID_ARG
+
+
 def test_int8_helpers_refuse_cpu_tensors():
     x, w = torch.zeros(4, 64), torch.ones(64)
     q, s = torch.zeros(4, 64, dtype=torch.int8), torch.ones(4)

@@ -11,6 +11,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <atomic>
 #include <functional>
 #include <queue>
 #include <vector>
@@ -89,11 +90,38 @@ int run_partial(const TmlaDecodeParams& p, cudaStream_t stream, bool part16 = fa
 
 }  // namespace
 
+// The library's own status word on each GPU (zero when the library is loaded there).
+static __device__ int32_t g_tmla_status;
+
 extern "C" {
 
 int tmla_abi_version(void) { return TMLA_ABI_VERSION; }
 
 size_t tmla_params_bytes(void) { return sizeof(TmlaDecodeParams); }
+
+int tmla_status_word(int32_t** word) {
+  // Its address on each device, looked up once.
+  constexpr int kDevices = 64;
+  static std::atomic<void*> known[kDevices];
+  if (!word) return TMLA_ERR_INVALID_ARG;
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return tmla::record_cuda_error(e);
+  void* at = device < kDevices ? known[device].load(std::memory_order_relaxed) : nullptr;
+  if (!at) {
+    // The lookup may load the library onto the device, which a capture by this thread would otherwise forbid.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return tmla::record_cuda_error(e);
+    e = cudaGetSymbolAddress(&at, g_tmla_status);
+    const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) e = back;
+    if (e != cudaSuccess) return tmla::record_cuda_error(e);
+    if (device < kDevices) known[device].store(at, std::memory_order_relaxed);
+  }
+  *word = static_cast<int32_t*>(at);
+  return TMLA_OK;
+}
 
 const char* tmla_error_string(int code) {
   switch (code) {

@@ -11,7 +11,7 @@
 //
 // Schema: decode(q [B, H, D], kv_cache [N, P, D], cache_seqlens int32 [B], block_table int32
 // [B, W] or None, out [B, H, Dv] (written), lse fp32 [B, H] (written), num_splits, softmax_scale,
-// kernel (TMLA_KERNEL_*), q_len, status int32 [1] or None) -> ().  The split workspace comes from
+// kernel (TMLA_KERNEL_*), q_len, status int32 [1], or None for the library's own word) -> ().  The split workspace comes from
 // the caching allocator on the current stream; the launches go on the current stream.
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -30,6 +30,20 @@ int32_t dtype_code(at::ScalarType t) {
     default: TORCH_CHECK(false, "triton_mla.decode: q must be bfloat16, float16 or float32, got ", t);
   }
   return -1;
+}
+
+void check_rc(int rc, const char* what) {
+  TORCH_CHECK(rc == TMLA_OK, what, " failed: ", tmla_error_string(rc), " ",
+              rc == TMLA_ERR_CUDA ? tmla_last_cuda_error() : "");
+}
+
+// The caller's status word, or the library's on the current device (what read_status reads: a call without one, as
+// torch.compile makes them, must not lose a timed-out wait).
+int32_t* status_word(const std::optional<at::Tensor>& status) {
+  if (status.has_value()) return status->data_ptr<int32_t>();
+  int32_t* word = nullptr;
+  check_rc(tmla_status_word(&word), "tmla_status_word");
+  return word;
 }
 
 void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& lens,
@@ -74,7 +88,6 @@ void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& le
   p.out_stride_h = out.stride(1);
   p.lse = lse.data_ptr<float>();
   p.lse_stride_b = lse.stride(0);
-  p.status = status.has_value() ? status->data_ptr<int32_t>() : nullptr;
   p.batch = (int32_t)B;
   p.num_heads = (int32_t)H;
   p.d_qk = (int32_t)D;
@@ -87,6 +100,7 @@ void decode_cuda(const at::Tensor& q, const at::Tensor& kv, const at::Tensor& le
   p.kv_format = fp8 ? TMLA_KV_FP8_E4M3 : TMLA_KV_SAME;
   if (B == 0) return;
   const c10::cuda::CUDAGuard guard(q.device());
+  p.status = status_word(status);
   const size_t ws_bytes = tmla_workspace_bytes(p.batch, p.num_heads, p.num_splits, p.d_v);
   at::Tensor ws;
   if (ws_bytes) {
@@ -127,11 +141,6 @@ void check_rows(const at::Tensor& t, const char* what) {
 }
 // A one-row matrix may carry any row stride, which nothing reads: one that breaks no alignment.
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : (t.size(1) + 15) / 16 * 16; }
-
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == TMLA_OK, what, " failed: ", tmla_error_string(rc), " ",
-              rc == TMLA_ERR_CUDA ? tmla_last_cuda_error() : "");
-}
 
 TmlaInt8RowsParams rows_params(const at::Tensor& x, const at::Tensor& q, const at::Tensor& scale, bool overlap) {
   TmlaInt8RowsParams p = {};
@@ -245,7 +254,7 @@ at::Tensor linear_int8_cuda(const at::Tensor& x, const at::Tensor& x_scale, cons
   p.n = (int32_t)w.size(0);
   p.k = (int32_t)x.size(1);
   p.dtype = dtype_code(out_dtype);
-  p.status = status.has_value() ? status->data_ptr<int32_t>() : nullptr;
+  p.status = status_word(status);
   p.flags = (overlap ? TMLA_LAYER_FLAG_PDL : 0) | TMLA_LINEAR_FLAG_PAD_Y;
   check_rc(tmla_linear_int8(&p, c10::cuda::getCurrentCUDAStream(x.device().index()).stream()), "tmla_linear_int8");
   return y;

@@ -74,6 +74,7 @@ EXPORTED = (
     "tmla_plan_units_device",
     "tmla_linear",
     "tmla_linear_workspace_bytes",
+    "tmla_status_word",
     "tmla_quantize_int8",
     "tmla_rms_norm_int8",
     "tmla_linear_int8",
@@ -319,6 +320,8 @@ def load() -> ctypes.CDLL:
     lib.tmla_abi_version.restype = ctypes.c_int
     lib.tmla_params_bytes.argtypes = []
     lib.tmla_params_bytes.restype = ctypes.c_size_t
+    lib.tmla_status_word.argtypes = [ctypes.POINTER(vp)]
+    lib.tmla_status_word.restype = ctypes.c_int
     lib.tmla_plan_units.argtypes = [vp, i32, i32, i32, i32, vp, vp]
     lib.tmla_plan_units.restype = i32
     lib.tmla_units_workspace_bytes.argtypes = [i32, i32, i32]

@@ -185,10 +185,23 @@ def get_num_splits(batch, num_heads, max_seqlen, num_sms, min_tokens_per_split=1
 _status = {}
 
 
+class _DeviceInt32:
+    """One int32 of device memory that is not PyTorch's, as its CUDA array interface describes it."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def _status_word(device: torch.device) -> torch.Tensor:
+    """The library's status word on ``device`` as a tensor.  It belongs to no allocator, so a call whose first use
+    of it is captured leaves nothing in the graph's memory pool."""
     t = _status.get(device.index)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=device)
+        word = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            _lib.check(_lib.load().tmla_status_word(ctypes.byref(word)), "tmla_status_word")
+            t = torch.as_tensor(_DeviceInt32(word.value), device=device)
+        assert t.data_ptr() == word.value, "a view of the library's word, not a copy"
         _status[device.index] = t
     return t
 

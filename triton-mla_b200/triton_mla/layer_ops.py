@@ -19,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .kernel import _DTYPE_CODES, _require_cuda, _status, _status_word
+from .kernel import _DTYPE_CODES, _require_cuda, _status_word
 
 
 def _stream(t: torch.Tensor):
@@ -255,14 +255,6 @@ def _check_linear_int8(x_q, x_scale, w_q, w_scale, out_dtype) -> None:
         raise TypeError(f"unsupported out_dtype {out_dtype}; use bfloat16, float16 or float32")
 
 
-def _int8_status(device):
-    """The device's status word, unless it would have to be made during a capture (in the graph's pool)."""
-    word = _status.get(device.index)
-    if word is None and device.type == "cuda" and not torch.cuda.is_current_stream_capturing():
-        word = _status_word(device)
-    return word
-
-
 def quantize_int8(x: torch.Tensor, overlap: bool = False):
     """int8 rows of ``x`` [m, k] with one scale each: ``(q, scale)`` with q int8 [m, k], scale
     fp32 [m] and ``x ~ q * scale[:, None]`` (C ABI: ``tmla_quantize_int8``).
@@ -317,7 +309,8 @@ def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_s
     is a multiple of 16 bytes).  Rows of x_q and w_q on 16-byte boundaries run on the tcgen05
     kernel, others on a much slower CUDA-core kernel with the same results.  ``overlap`` as in
     ``rms_norm_int8`` (the preceding kernel must not write ``w_q``)."""
-    status = None if torch.compiler.is_compiling() else _int8_status(x_q.device)
+    # None: the operator takes the library's status word itself.
+    status = None if torch.compiler.is_compiling() or not x_q.is_cuda else _status_word(x_q.device)
     try:
         return torch.ops.triton_mla.linear_int8(x_q, x_scale, w_q, w_scale, out_dtype, overlap, status)
     except (RuntimeError, TypeError):
