@@ -1,5 +1,5 @@
 """int8 rows (``layer_ops.quantize_int8``, ``rms_norm_int8``) at the borders of their definition: the integers bit for
-bit, rows of every kernel variant, products that pass fp32.
+bit, rows of every kernel variant, products that pass fp32, tensors that autograd watches.
 
 Tolerances of a norm, in units u = 2^-24 as in ``test_int8_gpu``, for every variant: a thread adds up to 64 squares
 in a row (8 vectors of 8 values, or k / 1024 + 8 for looped rows) and 10 more across threads.  rstd is off by half of
@@ -164,3 +164,21 @@ def test_eps_of_zero(device):
     q, s, _ = layer_ops.rms_norm_int8(x, w, 0.0)
     assert bool(torch.isnan(s[1])) and not bool(q[1].any())
     _check_norm(x[::2].contiguous(), w, 0.0)
+
+
+# ----------------------------------------------------------------------------- refusals
+def test_a_watched_tensor_is_not_written_in_place(device):
+    """Autograd cannot follow the operator, so a tensor that requires a gradient is not updated under it."""
+    x = torch.randn(4, 64, device=device)
+    w = torch.ones(64, device=device)
+    leaf = torch.randn(4, 64, device=device, requires_grad=True)
+    for watched in (leaf, leaf * 2):
+        before = watched.detach().clone()
+        with pytest.raises(RuntimeError, match="gradient"):
+            layer_ops.rms_norm_int8(x, w, residual=watched, residual_out=watched)
+        torch.cuda.synchronize()
+        assert torch.equal(watched.detach(), before)
+        with torch.no_grad():
+            want = (x + before)
+            _, _, h = layer_ops.rms_norm_int8(x, w, residual=watched, residual_out=watched)
+            assert h is watched and torch.equal(watched.detach(), want)

@@ -14,6 +14,7 @@
 // kernel (TMLA_KERNEL_*), q_len, status int32 [1], or None for the library's own word) -> ().  The split workspace comes from
 // the caching allocator on the current stream; the launches go on the current stream.
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -196,10 +197,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> rms_norm_int8_cuda(const at::Tens
   p.eps = (float)eps;
   if (residual.has_value()) {
     check_like(*residual, x, "residual");
-    if (residual_out.has_value())
+    if (residual_out.has_value()) {
       check_like(*residual_out, x, "residual_out");
-    else
+      TORCH_CHECK(!(c10::GradMode::is_enabled() && residual_out->requires_grad()),
+                  "triton_mla.rms_norm_int8: residual_out requires a gradient, which does not pass through this "
+                  "operator; call it under torch.no_grad()");
+    } else {
       h = aligned_rows(x.size(0), x.size(1), x.options(), x.scalar_type());
+    }
     const at::Tensor& out = residual_out.has_value() ? *residual_out : h;
     p.residual = residual->data_ptr();
     p.residual_stride = row_stride(*residual);

@@ -281,7 +281,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     ``h = x + residual`` rounded to x's dtype, ``y = h * weight / sqrt(mean(h^2) + eps)`` in fp32,
     and y's rows quantised as in ``quantize_int8``.  x [m, k] (any row stride), weight [k].  h is
     the new residual: a new tensor (rows on 16-byte boundaries, as q's), or ``residual_out``, which may be
-    ``residual`` or ``x`` itself (but overlap them in no other way).  Without a residual h is None
+    ``residual`` or ``x`` itself (but overlap them in no other way) and, outside ``torch.no_grad()``, must not
+    require a gradient (none passes through these operators).  Without a residual h is None
     and x is normalised as it is.  Squares that sum past fp32 (|h| above 1.8e19) make the norm 0,
     as any fp32 norm does: zeros with the smallest scale.  A NaN or an infinity in h or weight leaves a row without
     a scale (NaN, and zeros); a product h * weight past fp32 alone does not.
