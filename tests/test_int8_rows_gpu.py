@@ -182,3 +182,26 @@ def test_a_watched_tensor_is_not_written_in_place(device):
             want = (x + before)
             _, _, h = layer_ops.rms_norm_int8(x, w, residual=watched, residual_out=watched)
             assert h is watched and torch.equal(watched.detach(), want)
+
+
+def test_overlapping_rows_are_refused_by_name(device):
+    x = torch.randn(1, 64, device=device)
+    w = torch.ones(64, device=device)
+    wide = torch.randn(4, 64, device=device)
+    flat = torch.randn(400, device=device).as_strided((4, 64), (63, 1))
+    assert layer_ops.quantize_int8(x)[0].shape == (1, 64)
+    for rows in (x.expand(4, 64), flat):
+        with pytest.raises(AssertionError, match="row stride"):
+            layer_ops.quantize_int8(rows)
+        with pytest.raises(AssertionError, match="row stride"):
+            layer_ops.rms_norm_int8(rows, w)
+        with pytest.raises(AssertionError, match="row stride"):
+            layer_ops.rms_norm_int8(wide, w, residual=rows)
+        with pytest.raises(AssertionError, match="row stride"):
+            layer_ops.rms_norm_int8(wide, w, residual=wide, residual_out=rows)
+    q, s = layer_ops.quantize_int8(wide)
+    rows = q[:1].expand(4, 64)
+    with pytest.raises(AssertionError, match="row stride"):
+        layer_ops.linear_int8(rows, s, q, s)
+    with pytest.raises(AssertionError, match="row stride"):
+        layer_ops.linear_int8(q, s, rows, s)

@@ -223,12 +223,17 @@ def l2_prefetch(t: torch.Tensor, chunk_bytes: int = None, stride_bytes: int = No
 # The operators check their arguments themselves; these helpers name what is wrong with a refused call
 # in the package's own terms (a call that is accepted pays nothing for them: 9.5 -> 7 us of host
 # time per call).
+def _check_row_stride(t: torch.Tensor) -> None:
+    assert t.shape[0] < 2 or t.stride(0) >= t.shape[1], "overlapping rows (row stride below their length): copy them"
+
+
 def _check_int8_source(x: torch.Tensor) -> None:
     _require_cuda(x)
     if x.dtype not in _DTYPE_CODES:
         raise TypeError(f"unsupported dtype {x.dtype}; use bfloat16, float16 or float32")
     assert x.dim() == 2 and x.shape[1] > 0, "a matrix [m, k] with k >= 1"
     assert x.stride(1) == 1, "rows need unit inner stride"
+    _check_row_stride(x)
 
 
 def _check_rms_norm_int8(x, weight, residual, residual_out) -> None:
@@ -239,6 +244,7 @@ def _check_rms_norm_int8(x, weight, residual, residual_out) -> None:
     for t in (residual, residual_out):
         if t is not None:
             assert t.shape == x.shape and t.dtype == x.dtype and t.device == x.device and t.stride(1) == 1
+            _check_row_stride(t)
     assert residual is not None or residual_out is None, "residual_out without a residual"
 
 
@@ -247,6 +253,8 @@ def _check_linear_int8(x_q, x_scale, w_q, w_scale, out_dtype) -> None:
     assert x_q.dim() == 2 and w_q.dim() == 2 and x_q.shape[1] == w_q.shape[1] and x_q.shape[1] > 0
     assert x_q.dtype == torch.int8 and w_q.dtype == torch.int8, "int8 operands"
     assert x_q.stride(1) == 1 and w_q.stride(1) == 1, "rows need unit inner stride"
+    _check_row_stride(x_q)
+    _check_row_stride(w_q)
     assert x_scale.shape == x_q.shape[:1] and w_scale.shape == w_q.shape[:1], "a scale per token and per channel"
     assert x_scale.dtype == torch.float32 and w_scale.dtype == torch.float32
     assert x_scale.is_contiguous() and w_scale.is_contiguous()
@@ -264,7 +272,7 @@ def quantize_int8(x: torch.Tensor, overlap: bool = False):
     (a scale per token) and for weights [n, k] (a scale per output channel).  A row with a NaN
     or an infinity gets scale NaN and zeros.  Rows of q start on 16-byte boundaries, so q's row
     stride is k rounded up to 16 (the padding bytes are not written).  Bf16, fp16 or fp32, any
-    row stride; no gradient.  ``overlap`` as in ``rms_norm_int8`` (nothing to load early here)."""
+    row stride of at least k (expanded or overlapping rows are refused); no gradient.  ``overlap`` as in ``rms_norm_int8`` (nothing to load early here)."""
     try:
         return torch.ops.triton_mla.quantize_int8(x, overlap)
     except (RuntimeError, TypeError):
@@ -279,7 +287,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
     ``tmla_rms_norm_int8``).
 
     ``h = x + residual`` rounded to x's dtype, ``y = h * weight / sqrt(mean(h^2) + eps)`` in fp32,
-    and y's rows quantised as in ``quantize_int8``.  x [m, k] (any row stride), weight [k].  h is
+    and y's rows quantised as in ``quantize_int8``.  x [m, k] (any row stride >= k), weight [k].  h is
     the new residual: a new tensor (rows on 16-byte boundaries, as q's), or ``residual_out``, which may be
     ``residual`` or ``x`` itself (but overlap them in no other way) and, outside ``torch.no_grad()``, must not
     require a gradient (none passes through these operators).  Without a residual h is None
@@ -306,7 +314,7 @@ def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_s
     with fp32 scales per token and per output channel, as ``quantize_int8`` and ``rms_norm_int8``
     give them (C ABI: ``tmla_linear_int8``).  The products are summed exactly (int32, k at most
     131071) and scaled in fp32; y [m, n] is rounded once to ``out_dtype`` (bf16, fp16 or fp32).
-    Any m and n; no gradient.  Rows of y start on 16-byte boundaries (y is contiguous when a row
+    Any m and n, any row strides >= k; no gradient.  Rows of y start on 16-byte boundaries (y is contiguous when a row
     is a multiple of 16 bytes).  Rows of x_q and w_q on 16-byte boundaries run on the tcgen05
     kernel, others on a much slower CUDA-core kernel with the same results.  ``overlap`` as in
     ``rms_norm_int8`` (the preceding kernel must not write ``w_q``)."""
