@@ -442,6 +442,10 @@ typedef struct TmlaLinearInt8Params {
   int64_t wait_ns;                 /* limit of each pipeline wait (<= 0: 2 s) */
 } TmlaLinearInt8Params;
 int tmla_linear_int8(const TmlaLinearInt8Params* p, void* stream);
+/* The variant of the tcgen05 kernel that tmla_linear_int8 takes for these sizes on a GPU of num_sms SMs: plan[0] the CTAs
+   of a tile (1, or 2 for a pair), plan[1] its tokens, plan[2] the parts of k, plan[3] the tiles that the busiest CTA (or
+   pair) computes one after another.  Host-only. */
+int tmla_linear_int8_plan(int32_t m, int32_t n, int32_t k, int32_t dtype, int32_t num_sms, int32_t* plan);
 
 #ifdef __cplusplus
 }

@@ -277,6 +277,22 @@ def test_linear_int8_variants(device, m, n, k):
     assert read_status(device) == 0
 
 
+# The variants that the shapes above leave out, of fp32 output most of all: larger tiles of CTA pairs, split or not, and two
+# and three tiles in a row of each (``test_int8_host`` checks that the lists reach every variant of either output size).
+MORE_VARIANT_SHAPES = [
+    (38, 19579, 66), (54, 19048, 5624), (66, 20867, 68), (73, 20347, 3639), (105, 20043, 66),
+    (105, 20832, 2767), (135, 19542, 68), (193, 9671, 1834), (196, 3393, 10864), (224, 19019, 904),
+    (233, 19641, 813), (271, 4648, 13396), (282, 19390, 1374), (291, 10444, 1167), (332, 18948, 820),
+    (337, 15087, 65), (385, 2856, 8943), (400, 14673, 64), (417, 20003, 781), (524, 8343, 778), (673, 9756, 67),
+    (1597, 278, 5487), (2052, 280, 5766), (2458, 1896, 774), (3458, 3063, 777),
+]
+
+
+@pytest.mark.parametrize("m,n,k", MORE_VARIANT_SHAPES)
+def test_linear_int8_more_variants(device, m, n, k):
+    test_linear_int8_variants(device, m, n, k)
+
+
 @pytest.mark.parametrize("m,n,k,pad", [(5, 40, 100, 1), (70, 130, 257, 0), (16, 300, 1001, 2), (300, 65, 80, 3)])
 def test_linear_int8_rows_of_any_alignment(device, m, n, k, pad):
     """Rows that do not start on 16-byte boundaries (x, w or both) give the same values."""

@@ -137,3 +137,47 @@ def test_padded_rows_lie_in_their_own_storage(dtype, m, n):
         row = -(-n * t.element_size() // 16) * 16
         assert t.shape == (m, n) and t.stride(1) == 1 and (m < 2 or t.stride(0) * t.element_size() == max(row, t.element_size()))
         assert t.untyped_storage().nbytes() >= m * row and t.storage_offset() == 0 and not t._is_view()
+
+
+def _variant(m, n, k, dtype):
+    """(CTAs of a tile, tokens of a tile, parts of k, tiles in a row: 1, 2 or more) on 148 SMs."""
+    plan = (ctypes.c_int32 * 4)()
+    assert _lib.load().tmla_linear_int8_plan(m, n, k, dtype, 148, plan) == _lib.OK
+    return (*plan[:3], min(plan[3], 3))
+
+
+@pytest.mark.parametrize("dtype", [_lib.DTYPE_BF16, _lib.DTYPE_FP32])
+def test_the_gpu_tests_reach_every_variant_of_the_product(dtype):
+    """Whatever constants choose the variant: the shapes that the GPU tests run in every type reach all variants that
+    20,000 sizes (1 to 8192 tokens, spread over the logarithm) reach."""
+    import math
+    import random
+
+    import test_int8_gpu as gpu
+
+    rng = random.Random(11)
+
+    def log(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    run = {_variant(m, n, k, dtype) for m, n, k in gpu.LINEAR_SHAPES + gpu.VARIANT_SHAPES + gpu.MORE_VARIANT_SHAPES}
+    for _ in range(20000):
+        k = log(64, 16384)
+        size = (log(1, 8192), log(64, min(24576, 7168 * 16384 // k)), k)
+        assert _variant(*size, dtype) in run, (size, _variant(*size, dtype))
+
+
+@pytest.mark.parametrize("kw,code", [
+    (dict(m=0), _lib.ERR_INVALID_ARG),
+    (dict(n=0), _lib.ERR_INVALID_ARG),
+    (dict(k=0), _lib.ERR_INVALID_ARG),
+    (dict(dtype=3), _lib.ERR_INVALID_ARG),
+    (dict(num_sms=0), _lib.ERR_INVALID_ARG),
+    (dict(plan=None), _lib.ERR_INVALID_ARG),
+    (dict(m=(1 << 30) + 1), _lib.ERR_UNSUPPORTED),
+    (dict(k=_lib.LINEAR_INT8_MAX_K + 1), _lib.ERR_UNSUPPORTED),
+])
+def test_the_plan_checks_its_arguments(kw, code):
+    args = dict(m=1, n=1, k=1, dtype=_lib.DTYPE_BF16, num_sms=148, plan=(ctypes.c_int32 * 4)())
+    args.update(kw)
+    assert _lib.load().tmla_linear_int8_plan(*args.values()) == code

@@ -961,6 +961,21 @@ int start(const TmlaLinearInt8Params& p, cudaStream_t stream) {
 }  // namespace linear_int8
 }  // namespace tmla
 
+extern "C" int tmla_linear_int8_plan(int32_t m, int32_t n, int32_t k, int32_t dtype, int32_t num_sms, int32_t* plan) {
+  using namespace tmla::linear_int8;
+  if (m < 1 || n < 1 || k < 1 || num_sms < 1 || !plan) return TMLA_ERR_INVALID_ARG;
+  if (dtype != TMLA_DTYPE_BF16 && dtype != TMLA_DTYPE_FP16 && dtype != TMLA_DTYPE_FP32) return TMLA_ERR_INVALID_ARG;
+  if (k > TMLA_LINEAR_INT8_MAX_K || m > kMaxRows || n > kMaxRows) return TMLA_ERR_UNSUPPORTED;
+  const Plan p = make_plan(m, n, k, dtype == TMLA_DTYPE_FP32 ? 4 : 2, num_sms);
+  const long long tiles = (long long)((n + kRows * p.group - 1) / (kRows * p.group)) * ((m + p.tok - 1) / p.tok);
+  const long long slots = num_sms / p.group;
+  plan[0] = p.group;
+  plan[1] = p.tok;
+  plan[2] = p.splits;
+  plan[3] = p.splits > 1 ? 1 : (int)((tiles + slots - 1) / slots);
+  return TMLA_OK;
+}
+
 extern "C" int tmla_linear_int8(const TmlaLinearInt8Params* p, void* stream) {
   if (!p) return TMLA_ERR_INVALID_ARG;
   return tmla::linear_int8::start(*p, static_cast<cudaStream_t>(stream));

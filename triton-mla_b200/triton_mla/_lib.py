@@ -78,6 +78,7 @@ EXPORTED = (
     "tmla_quantize_int8",
     "tmla_rms_norm_int8",
     "tmla_linear_int8",
+    "tmla_linear_int8_plan",
 )
 
 
@@ -339,6 +340,8 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(st), vp]
         fn.restype = ctypes.c_int
+    lib.tmla_linear_int8_plan.argtypes = [i32, i32, i32, i32, i32, ctypes.POINTER(i32)]
+    lib.tmla_linear_int8_plan.restype = ctypes.c_int
     lib.tmla_l2_prefetch.argtypes = [vp, i64, i64, i32, i32, vp]
     lib.tmla_l2_prefetch.restype = ctypes.c_int
     if lib.tmla_abi_version() != ABI_VERSION:
