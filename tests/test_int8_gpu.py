@@ -667,3 +667,55 @@ def test_timed_out_parts_of_a_split_tile(device, m, n, k):
         torch.cuda.synchronize()
         assert read_status(device) == _lib.STATUS_TIMEOUT
         _compare_linear(y2, xq, xs, wq, ws)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 7211), (16, 2112, 7168), (300, 520, 1024), (5, 40, 99)])
+def test_linear_int8_scales_without_a_value(device, m, n, k):
+    """A token or channel whose scale is infinite or NaN (a row without one) has no finite product, in split tiles, in
+    whole ones and in rows of y off 16-byte boundaries; the others are exact."""
+    g = _gen(device, 41)
+    xq, wq = _int8(m, k, g, device), _int8(n, k, g, device)
+    xs, ws = torch.rand(m, generator=g, device=device) + 0.01, torch.rand(n, generator=g, device=device) + 0.01
+    for dtype in DTYPES:
+        want = layer_ops.linear_int8(xq, xs, wq, ws, dtype)
+        bad_x, bad_w = xs.clone(), ws.clone()
+        bad_x[m - 1], bad_w[1], bad_w[n - 1] = float("nan"), float("inf"), float("nan")
+        assert bool(torch.isnan(layer_ops.linear_int8(xq, bad_x, wq, ws, dtype)[m - 1]).all())
+        if m > 1:
+            assert torch.equal(layer_ops.linear_int8(xq, bad_x, wq, ws, dtype)[: m - 1], want[: m - 1])
+        y = layer_ops.linear_int8(xq, xs, wq, bad_w, dtype)
+        assert not bool(torch.isfinite(y[:, [1, n - 1]]).any())
+        assert torch.equal(y[:, 2:n - 1], want[:, 2:n - 1]) and torch.equal(y[:, 0], want[:, 0])
+    assert read_status(device) == 0
+
+
+def test_an_in_place_residual_under_torch_compile(device):
+    def f(x, r, w):
+        q, s, h = layer_ops.rms_norm_int8(x, w, residual=r, residual_out=r)
+        return q, s, h + 1
+
+    g = _gen(device, 42)
+    x, r = (torch.randn(5, 200, generator=g, device=device).to(torch.bfloat16) for _ in range(2))
+    w = torch.ones(200, device=device, dtype=torch.bfloat16)
+    r1, r2 = r.clone(), r.clone()
+    got, want = torch.compile(f, fullgraph=True, backend="aot_eager")(x, r1, w), f(x, r2, w)
+    assert torch.equal(r1, r2) and torch.equal(r1, x + r)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_of_another_device_than_the_current_one(device):
+    other = torch.device("cuda", 1)
+    g = _gen(other, 43)
+    x = torch.randn(9, 1001, generator=g, device=other)
+    w = torch.ones(1001, device=other)
+    wq, ws = layer_ops.quantize_int8(torch.randn(70, 1001, generator=g, device=other))
+    with torch.cuda.device(0):
+        q, s, h = layer_ops.rms_norm_int8(x, w, residual=x)
+        y = layer_ops.linear_int8(q, s, wq, ws, torch.float32)
+        assert torch.cuda.current_device() == 0
+    assert {t.device for t in (q, s, h, y)} == {other}
+    torch.cuda.synchronize(other)
+    _compare_linear(y, q, s, wq, ws)
+    assert read_status(other) == 0
