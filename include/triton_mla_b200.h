@@ -423,8 +423,8 @@ int tmla_rms_norm_int8(const TmlaInt8RowsParams* p, void* stream);
    makes the first CTA skip its first loads). */
 #define TMLA_LINEAR_INT8_MAX_K 131071
 /* The bytes of a row of y from column n to the next 16-byte boundary may be written: y_stride covers
-   them, and the memory of y does so behind the last row too (m * y_stride values).  With n not a multiple of 16 bytes, rows on 16-byte boundaries can then be stored by TMA,
-   about twice as fast. */
+   them, and the memory of y does so behind the last row too (m * y_stride values).  With n not a
+   multiple of 16 bytes, rows on 16-byte boundaries can then be stored by TMA, about twice as fast. */
 #define TMLA_LINEAR_FLAG_PAD_Y 0x2
 typedef struct TmlaLinearInt8Params {
   const void* x;                   /* int8 [m, k] */

@@ -135,7 +135,8 @@ def test_padded_rows_lie_in_their_own_storage(dtype, m, n):
         tensors += [q, h, ops.quantize_int8(x, False)[0]]
     for t in tensors:
         row = -(-n * t.element_size() // 16) * 16
-        assert t.shape == (m, n) and t.stride(1) == 1 and (m < 2 or t.stride(0) * t.element_size() == max(row, t.element_size()))
+        assert t.shape == (m, n) and t.stride(1) == 1
+        assert m < 2 or t.stride(0) * t.element_size() == max(row, t.element_size())
         assert t.untyped_storage().nbytes() >= m * row and t.storage_offset() == 0 and not t._is_view()
 
 

@@ -7,8 +7,9 @@
 // The scale needs max |y| and the norm needs sum h^2, but rstd is one positive factor of the whole
 // row: max_j |h_j w_j rstd| = rstd max_j |h_j w_j| (rounding is monotone).  So both reductions
 // run at once over the row, which stays in registers, and every input is read and every
-// output written exactly once (rows too long for a block's registers are read twice, see loop_kernel).  Arithmetic is fp32 whatever T is; h is rounded to T first (the
-// norm is of the residual stream as stored), the int8 values are rounded once, to nearest even.
+// output written exactly once (rows too long for a block's registers are read twice, see loop_kernel).
+// Arithmetic is fp32 whatever T is; h is rounded to T first (the norm is of the residual stream as
+// stored), the integers are rounded to nearest even.
 //
 // Bound: HBM bandwidth.  Measured on B200 (inputs beyond L2, back to back): quantise 8192 x 7168 bf16
 // 28.3 us (6.2 TB/s, 95% of a copy), norm with residual 70 us (5.9 TB/s, 90%), norm without

@@ -11,8 +11,9 @@
 //
 // Schema: decode(q [B, H, D], kv_cache [N, P, D], cache_seqlens int32 [B], block_table int32
 // [B, W] or None, out [B, H, Dv] (written), lse fp32 [B, H] (written), num_splits, softmax_scale,
-// kernel (TMLA_KERNEL_*), q_len, status int32 [1], or None for the library's own word) -> ().  The split workspace comes from
-// the caching allocator on the current stream; the launches go on the current stream.
+// kernel (TMLA_KERNEL_*), q_len, status int32 [1], or None for the library's own word) -> ().  The
+// split workspace comes from the caching allocator on the current stream; the launches go on the
+// current stream.
 #include <ATen/ATen.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>

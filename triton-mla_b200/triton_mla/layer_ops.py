@@ -272,7 +272,8 @@ def quantize_int8(x: torch.Tensor, overlap: bool = False):
     (a scale per token) and for weights [n, k] (a scale per output channel).  A row with a NaN
     or an infinity gets scale NaN and zeros.  Rows of q start on 16-byte boundaries, so q's row
     stride is k rounded up to 16 (the padding bytes are not written).  Bf16, fp16 or fp32, any
-    row stride of at least k (expanded or overlapping rows are refused); no gradient.  ``overlap`` as in ``rms_norm_int8`` (nothing to load early here)."""
+    row stride of at least k (expanded or overlapping rows are refused); no gradient.  ``overlap``
+    as in ``rms_norm_int8`` (nothing to load early here)."""
     try:
         return torch.ops.triton_mla.quantize_int8(x, overlap)
     except (RuntimeError, TypeError):
@@ -316,8 +317,8 @@ def linear_int8(x_q: torch.Tensor, x_scale: torch.Tensor, w_q: torch.Tensor, w_s
     131071) and scaled in fp32; y [m, n] is rounded once to ``out_dtype`` (bf16, fp16 or fp32).
     Any m and n, any row strides >= k; no gradient.  Rows of y start on 16-byte boundaries (y is contiguous when a row
     is a multiple of 16 bytes).  Rows of x_q and w_q on 16-byte boundaries run on the tcgen05
-    kernel, others on a much slower CUDA-core kernel with the same results (500 x 4001 x 2001: 389 us, aligned 8.8).  ``overlap`` as in
-    ``rms_norm_int8`` (the preceding kernel must not write ``w_q``)."""
+    kernel, others on a much slower CUDA-core kernel with the same results (500 x 4001 x 2001: 389 us,
+    aligned 8.8).  ``overlap`` as in ``rms_norm_int8`` (the preceding kernel must not write ``w_q``)."""
     # None: the operator takes the library's status word itself.
     status = None if torch.compiler.is_compiling() or not x_q.is_cuda else _status_word(x_q.device)
     try:
